@@ -409,6 +409,54 @@ SB200_API int sb200_stream_triad_f32(int dev, uint64_t stream, uint64_t a, uint6
  * the intermediate is eliminated (sarek/sarek/Sarek_fusion.ml:490-499). */
 SB200_API int sb200_chain_triad_square_f32(int dev, uint64_t stream, uint64_t d, uint64_t a_out, uint64_t b, uint64_t c, float scalar, int64_t n);
 
+/* ---- microscaled matrices: 8 or 4 bits a value, a power-of-two scale for every 32 -------------------
+ * What a network's layers are trained and served in: activations and weights as e4m3 or e2m1 values with a scale of type e8m0 (2^(byte - 127),
+ * 255: NaN) for every 32 along K, the dimension that a product sums over.  A matrix of `rows` x K lies in two buffers of the caller's:
+ *   codes   row by row, each row padded with zeros to a multiple of 128 values: SB200_MX_FP8 a byte a value, SB200_MX_FP4 two values a
+ *           byte, the first in the low half.
+ *   scales  tiles of 128 rows x 4 scales, 512 bytes each, row after row of tiles: the scale of row r and block b (values 32b ..) is byte
+ *           (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4 of tile (r / 128) * ceil(K / 128) + b / 4.  Zero past the last row and K.
+ * Both start on 32 bytes (SB200_ERR_ALIGNMENT).  The scale of a block is 2^max(floor(log2 m) - e, -127), m the largest magnitude in it, e = 8
+ * for e4m3 and 2 for e2m1; values are rounded to the nearest, ties to even, and held at the type's largest (448, 6).  A block with a
+ * NaN or an infinity gets the scale NaN.  As with the other direct operators, calls may be issued on any streams, buffers of this
+ * library are checked for their extent, and a call enqueues nothing but kernel launches; these use no scratch of the library's, so that
+ * calls on several streams run side by side and graphs of them may be replayed side by side. */
+#define SB200_MX_FP8 8
+#define SB200_MX_FP4 4
+/* Bytes of the two buffers. */
+SB200_API int sb200_mx_bytes(int format, int64_t rows, int64_t K, uint64_t *codes, uint64_t *scales);
+/* A float32 matrix to a microscaled one: src is rows x K with leading dimension ld, or K x rows if `transposed` (a weight matrix stored
+ * K x N becomes the N x K operand of a product; a gradient becomes the operand of either of its two products). */
+SB200_API int sb200_mx_quantize(int dev, uint64_t stream, int format, int64_t rows, int64_t K, uint64_t src, int64_t ld,
+                                int transposed, uint64_t codes, uint64_t scales);
+/* The values of a microscaled matrix, exactly. */
+SB200_API int sb200_mx_dequantize(int dev, uint64_t stream, int format, int64_t rows, int64_t K, uint64_t codes, uint64_t scales,
+                                  uint64_t dst, int64_t ld);
+/* D[M x N] = act(alpha * A[M x K] . B[N x K]^T + beta * C[M x N] + bias[N]) of microscaled A and B in either format each, the sums float32;
+ * D, C and bias as in sb200_gemm_f32 (C and bias may be 0, D may be C).  Gradients of y = x . W^T: dx = dy . W takes dy and W quantised along
+ * N, dW = dy^T . x takes both quantised along M (`transposed`). */
+SB200_API int sb200_gemm_mx(int dev, uint64_t stream, int format_a, int format_b, int64_t M, int64_t N, int64_t K,
+                            uint64_t a_codes, uint64_t a_scales, uint64_t b_codes, uint64_t b_scales,
+                            uint64_t D, int64_t ldd, float alpha, uint64_t C, int64_t ldc, float beta, uint64_t bias, int act);
+
+/* ---- root-mean-square norm ----------------------------------------------------------------------------
+ * h = x + residual (rounded to float32; residual may be 0), y = h * weight / sqrt(mean(h^2) + eps), by rows of `cols`.  Results, each
+ * optional: `sum` takes h, y the float32 result, codes and scales (format SB200_MX_FP8 or SB200_MX_FP4; 0: none) the microscaled one, whose
+ * codes are roundings of y in 64 bits.  sum may be x or residual, y may be x, residual or sum, each at the same leading dimension. */
+SB200_API int sb200_rmsnorm_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint64_t x, int64_t ldx, uint64_t residual, int64_t ldr,
+                                uint64_t weight, double eps, uint64_t sum, int64_t lds, uint64_t y, int64_t ldy,
+                                int format, uint64_t codes, uint64_t scales);
+/* Its gradient: with r = 1 / sqrt(mean(sum^2) + eps), n = sum * r and g = dy * weight,
+ *   dx = dsum + r * (g - n * mean(g * n))  (the gradient of x and of residual),  dweight = sum over the rows of dy * n,
+ * dsum the gradient that reaches `sum` from elsewhere (may be 0).  dx or dweight may be 0; dx may be dy, dsum or sum at the same leading
+ * dimension.  dweight needs a workspace of sb200_rmsnorm_workspace_bytes: min(rows, 512) * cols * 4; calls that may run at the same
+ * time need one each.  Results do not depend on timing. */
+#define SB200_RMSNORM_MAX_PARTS 512
+SB200_API int sb200_rmsnorm_workspace_bytes(int64_t rows, int64_t cols, uint64_t *bytes);
+SB200_API int sb200_rmsnorm_backward_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint64_t sum, int64_t lds, uint64_t weight,
+                                         double eps, uint64_t dy, int64_t lddy, uint64_t dsum, int64_t ldds, uint64_t dx, int64_t lddx,
+                                         uint64_t dweight, uint64_t workspace, uint64_t workspace_bytes);
+
 /* default numeric mode for GEMM kernels launched through sb200_kernel_launch
  * (also read once from the environment variable SAREK_B200_MODE=3xtf32|tf32|3xf16|f16) */
 SB200_API int sb200_set_mode(int mode);

@@ -20,6 +20,7 @@ SHARD_GATHER_FUSED, SHARD_GATHER_NCCL, SHARD_B_RESIDENT = 1, 2, 4
 MODE_3XTF32, MODE_TF32, MODE_3XF16, MODE_F16, MODE_3XMIXED = 3, 1, 4, 2, 5
 ACT_NONE, ACT_RELU = 0, 1
 KIND_MAP, KIND_GEMM_NAIVE, KIND_GEMM_TILED, KIND_BLOCK_REDUCE = 1, 2, 3, 4
+MX_FP8, MX_FP4 = 8, 4
 ARG_BUFFER, ARG_I32, ARG_I64, ARG_F32, ARG_F64 = 0, 1, 2, 3, 4
 
 
@@ -109,6 +110,13 @@ SIGNATURES = {
     "sb200_vector_add_f32": ([i32, u64, u64, u64, u64, i64], i32),
     "sb200_stream_triad_f32": ([i32, u64, u64, u64, u64, f32, i64], i32),
     "sb200_chain_triad_square_f32": ([i32, u64, u64, u64, u64, u64, f32, i64], i32),
+    "sb200_mx_bytes": ([i32, i64, i64, p(u64), p(u64)], i32),
+    "sb200_mx_quantize": ([i32, u64, i32, i64, i64, u64, i64, i32, u64, u64], i32),
+    "sb200_mx_dequantize": ([i32, u64, i32, i64, i64, u64, u64, u64, i64], i32),
+    "sb200_gemm_mx": ([i32, u64, i32, i32, i64, i64, i64, u64, u64, u64, u64, u64, i64, f32, u64, i64, f32, u64, i32], i32),
+    "sb200_rmsnorm_f32": ([i32, u64, i64, i64, u64, i64, u64, i64, u64, f64, u64, i64, u64, i64, i32, u64, u64], i32),
+    "sb200_rmsnorm_workspace_bytes": ([i64, i64, p(u64)], i32),
+    "sb200_rmsnorm_backward_f32": ([i32, u64, i64, i64, u64, i64, u64, f64, u64, i64, u64, i64, u64, i64, u64, u64, u64], i32),
     "sb200_set_mode": ([i32], i32),
     "sb200_get_mode": ([p(i32)], i32),
     "sb200_set_gemm_variant": ([i32], i32),

@@ -1,10 +1,56 @@
 // internal.hpp — what the library's translation units share besides the public C ABI.
 #pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <utility>
+
+#include "../../include/sb200.h"
 
 namespace sb200 {
 
 // Records a failure for sb200_last_error_string() on the calling thread and returns `code`.
 int set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+
+// A failed CUDA call, as a status.
+int set_cuda_error(cudaError_t e, const char* what);
+
+// What an operator outside sb200_shim.cu needs of a device.
+struct OperatorDevice {
+  int index, sm_count;
+  int* status;  // device word for kernels whose bounded waits expire; operator_waits() before such a launch
+};
+int operator_device(int dev, OperatorDevice* out);  // makes it the calling thread's current device
+void operator_waits(int dev);                       // a synchronise has the status word to read from now on
+int operator_extent(int dev, uint64_t ptr, uint64_t bytes, const char* what);  // SB200_ERR_BOUNDS past the end of a buffer of the library
+int operator_launched(const char* what);            // counts a launch, or reports that it failed
+int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t rows, uint64_t row_bytes,
+                         uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle);
+
+// Launches a kernel with programmatic stream serialization: it may set itself up while the kernel before it in the stream
+// still runs.  Every kernel launched this way passes griddepcontrol.wait before it touches global memory.  The launch call
+// itself is cheaper too (2.3 against 2.8 us).
+template <class... Params, class... Args>
+cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, Args&&... args) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof cfg);
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
 
 // The numeric modes every GEMM entry point takes.
 inline bool valid_mode(int mode) {

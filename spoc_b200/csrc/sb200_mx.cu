@@ -1,0 +1,404 @@
+// sb200_mx.cu — the C ABI of the microscaled operators and the root-mean-square norm (include/sb200.h): argument checks, the choice of a
+// kernel's form, launches.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <limits.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "../../include/sb200.h"
+#include "gemm_mx.cuh"
+#include "internal.hpp"
+#include "microscale.cuh"
+#include "rmsnorm.cuh"
+
+using namespace sb200;
+
+namespace {
+
+constexpr int kMaxDevices = 16;
+constexpr int64_t kMaxDim = 0x7fffffffLL - 128;
+
+#define CU_TRY(call)                                           \
+  do {                                                         \
+    cudaError_t e__ = (call);                                  \
+    if (e__ != cudaSuccess) return set_cuda_error(e__, #call); \
+  } while (0)
+
+inline cudaStream_t as_stream(uint64_t s) { return reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(s)); }
+template <class T>
+T* as_ptr(uint64_t p) {
+  return reinterpret_cast<T*>(static_cast<uintptr_t>(p));
+}
+bool on_16(uint64_t p, int64_t ld) { return (p & 15) == 0 && (ld & 3) == 0; }
+
+bool known_format(int format) { return format == SB200_MX_FP8 || format == SB200_MX_FP4; }
+int64_t chunks_of(int64_t K) { return (K + MX_CHUNK - 1) / MX_CHUNK; }
+uint64_t code_bytes(int format, int64_t rows, int64_t K) {
+  return static_cast<uint64_t>(rows) * chunks_of(K) * (format == SB200_MX_FP4 ? 64 : 128);
+}
+uint64_t scale_bytes(int64_t rows, int64_t K) { return static_cast<uint64_t>((rows + 127) / 128) * chunks_of(K) * MX_TILE_BYTES; }
+
+int check_shape(int64_t rows, int64_t K, const char* what) {
+  if (rows < 0 || K < 0) return set_error(SB200_ERR_INVALID_VALUE, "%s: negative dimension (%lld x %lld)", what, (long long)rows, (long long)K);
+  if (rows > kMaxDim || K > kMaxDim) return set_error(SB200_ERR_TOO_LARGE, "%s: dimension beyond 2^31 (%lld x %lld)", what, (long long)rows, (long long)K);
+  // tiles of scales are counted in 32 bits
+  if (static_cast<uint64_t>((rows + 127) / 128) * chunks_of(K) > 0x7fffffffull)
+    return set_error(SB200_ERR_TOO_LARGE, "%s: %lld x %lld has more than 2^31 - 1 tiles of scales", what, (long long)rows, (long long)K);
+  return SB200_OK;
+}
+int check_format(int format) {
+  return known_format(format) ? SB200_OK : set_error(SB200_ERR_INVALID_VALUE, "unknown microscaled format %d", format);
+}
+// A microscaled operand that is there: both buffers, where TMA can read them, inside their allocations.
+int check_mx(int dev, int format, int64_t rows, int64_t K, uint64_t codes, uint64_t scales, const char* what) {
+  if (!codes || !scales) return set_error(SB200_ERR_INVALID_VALUE, "%s: null codes or scales", what);
+  if ((codes | scales) & 31) return set_error(SB200_ERR_ALIGNMENT, "%s: codes and scales start on 32 bytes", what);
+  if (int rc = operator_extent(dev, codes, code_bytes(format, rows, K), what)) return rc;
+  return operator_extent(dev, scales, scale_bytes(rows, K), what);
+}
+// A float32 matrix that is there.
+int check_matrix(int dev, uint64_t p, int64_t rows, int64_t cols, int64_t ld, const char* what) {
+  if (!p) return set_error(SB200_ERR_INVALID_VALUE, "%s: null device pointer", what);
+  if (p & 3) return set_error(SB200_ERR_ALIGNMENT, "%s: float32 matrices must be 4-byte aligned", what);
+  if (ld < cols) return set_error(SB200_ERR_INVALID_VALUE, "%s: leading dimension %lld smaller than the row length %lld", what, (long long)ld, (long long)cols);
+  if (ld > INT64_MAX / 8 / (rows > 0 ? rows : 1)) return set_error(SB200_ERR_TOO_LARGE, "%s: extent beyond 64 bits", what);
+  return rows && cols ? operator_extent(dev, p, (static_cast<uint64_t>(rows - 1) * ld + cols) * 4, what) : SB200_OK;
+}
+
+// Blocks for `work` units, `per_block` each, at most `waves` waves of what fits a chip.
+unsigned grid_for(int64_t work, int64_t per_block, int64_t cap) {
+  const int64_t blocks = (work + per_block - 1) / per_block;
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min(blocks, cap)));
+}
+
+// ------------------------------------------------------------------ norm
+template <int FORMAT, bool VEC>
+int launch_rmsnorm(cudaStream_t st, const RmsNorm& p) {
+  const int64_t rows = FORMAT ? (p.rows + 127) / 128 * 128 : p.rows;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(rows, 0x7fffffff));
+  // the fewest float4 a thread that hold the row, in blocks of up to 1024 threads
+#define SB200_NORM(THREADS, VECS) CU_TRY(launch_pdl(rmsnorm_kernel<FORMAT, THREADS, VECS, VEC>, dim3(grid), dim3(THREADS), 0, st, 1, p))
+  const int64_t cols = p.cols;
+  if (cols <= 512) SB200_NORM(128, 1);
+  else if (cols <= 1024) SB200_NORM(256, 1);
+  else if (cols <= 2048) SB200_NORM(256, 2);
+  else if (cols <= 4096) SB200_NORM(256, 4);
+  else if (cols <= 8192) SB200_NORM(512, 4);
+  else if (cols <= 16384) SB200_NORM(512, 8);
+  else if (cols <= 32768) SB200_NORM(1024, 8);
+  else SB200_NORM(1024, 0);
+#undef SB200_NORM
+  return operator_launched("rmsnorm_kernel");
+}
+
+template <bool VEC>
+int launch_rmsnorm_backward(cudaStream_t st, const RmsNormBackward& p, unsigned grid) {
+#define SB200_NORM(THREADS, VECS) CU_TRY(launch_pdl(rmsnorm_backward_kernel<THREADS, VECS, VEC>, dim3(grid), dim3(THREADS), 0, st, 1, p))
+  const int64_t cols = p.cols;
+  if (cols <= 512) SB200_NORM(128, 1);
+  else if (cols <= 1024) SB200_NORM(256, 1);
+  else if (cols <= 2048) SB200_NORM(256, 2);
+  else if (cols <= 4096) SB200_NORM(256, 4);
+  else if (cols <= 8192) SB200_NORM(512, 4);
+  else if (cols <= 16384) SB200_NORM(512, 8);
+  else SB200_NORM(1024, 0);
+#undef SB200_NORM
+  if (int rc = operator_launched("rmsnorm_backward_kernel")) return rc;
+  if (!p.dweight) return SB200_OK;
+  CU_TRY(launch_pdl(rmsnorm_dweight_kernel, dim3(grid_for(p.cols, 32, 1 << 20)), dim3(256), 0, st, 1, static_cast<const float*>(p.workspace),
+                    static_cast<int>(grid), p.dweight, static_cast<long long>(p.cols)));
+  return operator_launched("rmsnorm_dweight_kernel");
+}
+int64_t dweight_parts(int64_t rows) { return std::min<int64_t>(rows, SB200_RMSNORM_MAX_PARTS); }
+
+// --------------------------------------------------------------- product
+// Tiles: 128 (256: pairs) columns of D by bt rows.
+struct MxShape {
+  int ctas = 1, bt = 128, splits = 1;
+};
+int64_t mx_tiles(const MxShape& s, int64_t M, int64_t N) { return (N + 128 * s.ctas - 1) / (128 * s.ctas) * ((M + s.bt - 1) / s.bt); }
+
+MxShape choose_mx_shape(int64_t M, int64_t N, int64_t k_blocks, int sm_count) {
+  MxShape s;
+  if (M <= 128) {
+    s.bt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  } else {
+    s.ctas = 2;
+    s.bt = 256;
+    if (mx_tiles(s, M, N) < sm_count / 2) s.bt = 128;
+    if (mx_tiles(s, M, N) < sm_count / 2) s.ctas = 1;
+  }
+  if (s.ctas == 1) {
+    const int64_t tiles = mx_tiles(s, M, N);
+    while (s.splits < 8 && tiles * s.splits * 2 <= sm_count && k_blocks >= s.splits * 4) s.splits *= 2;
+  }
+  return s;
+}
+
+template <bool FP4, int CTAS>
+int launch_mx(const OperatorDevice& d, cudaStream_t st, const CUtensorMap (&maps)[4], const MxGemm& p) {
+  auto kernel = gemm_mx_kernel<FP4, CTAS>;
+  constexpr int kSmem = 1024 + MXG_CTRL_BYTES + MXG_RING_BYTES;
+  static std::atomic<bool> ready[kMaxDevices];
+  if (!ready[d.index].load()) {
+    CU_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    ready[d.index].store(true);
+  }
+  const int tiles = p.tiles_f * p.tiles_t, units = d.sm_count / CTAS;
+  const int grid = p.splits > 1 ? tiles * p.splits : CTAS * std::min(tiles, units);
+  operator_waits(d.index);
+  CU_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(MXG_THREADS), kSmem, st, CTAS * p.splits, maps[0], maps[1], maps[2], maps[3], p));
+  return operator_launched("gemm_mx_kernel");
+}
+
+int run_gemm_mx(const OperatorDevice& d, cudaStream_t st, int format_a, int format_b, int64_t K, uint64_t a_codes, uint64_t a_scales, uint64_t b_codes,
+                uint64_t b_scales, MxGemm p) {
+  const bool fp4 = format_a == SB200_MX_FP4 && format_b == SB200_MX_FP4;
+  p.chunks = static_cast<int>(chunks_of(K));
+  p.num_k_blocks = fp4 ? (p.chunks + 1) / 2 : p.chunks;
+  const MxShape s = choose_mx_shape(p.M, p.N, p.num_k_blocks, d.sm_count);
+  const int64_t tiles = mx_tiles(s, p.M, p.N);
+  if (tiles > INT_MAX / 16) return set_error(SB200_ERR_TOO_LARGE, "gemm_mx: %lld tiles", (long long)tiles);
+  p.bt = s.bt;
+  p.tiles_f = static_cast<int>((p.N + 128ll * s.ctas - 1) / (128 * s.ctas));
+  p.tiles_t = static_cast<int>((p.M + static_cast<int64_t>(s.bt) - 1) / s.bt);
+  p.groups = s.bt > 128 ? 2 : 1;
+  p.split_k_blocks = (p.num_k_blocks + s.splits - 1) / s.splits;
+  p.splits = (p.num_k_blocks + p.split_k_blocks - 1) / p.split_k_blocks;  // the last one has something to do
+  const int scale_tiles = fp4 ? 2 : 1;
+  const int x_bytes = s.bt / s.ctas * 128, sf_bytes = scale_tiles * MX_TILE_BYTES * (1 + p.groups);
+  p.stage_bytes = (static_cast<int>(MXG_W_BYTES) + x_bytes + sf_bytes + 1023) / 1024 * 1024;
+  p.stages = std::min(MXG_MAX_STAGES, MXG_RING_BYTES / p.stage_bytes);
+  p.accs = 2 * s.bt + 2 * 4 * scale_tiles * (1 + p.groups) <= MXG_TMEM_COLS ? 2 : 1;
+  // spread: 4-bit codes that TMA spreads to a byte a value; a barrier counts the bytes that it reads
+  const bool spread_w = !fp4 && format_b == SB200_MX_FP4, spread_x = !fp4 && format_a == SB200_MX_FP4;
+  p.tx_bytes = s.ctas * ((static_cast<int>(MXG_W_BYTES) >> (spread_w ? 1 : 0)) + (x_bytes >> (spread_x ? 1 : 0)) + sf_bytes);
+  p.idesc = umma_idesc_mx(128u * s.ctas, static_cast<uint32_t>(s.bt), fp4 ? 1u : format_b == SB200_MX_FP4 ? 5u : 0u,
+                          fp4 ? 1u : format_a == SB200_MX_FP4 ? 5u : 0u);
+  p.status = d.status;
+  CUtensorMap maps[4];
+  auto codes_map = [&](CUtensorMap* map, uint64_t codes, int format, int64_t rows, bool spread, int box_rows) {
+    const uint64_t row_bytes = static_cast<uint64_t>(p.chunks) * (format == SB200_MX_FP4 ? 64 : 128);
+    return encode_tensor_map_2d(map, spread ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, as_ptr<void>(codes),
+                                spread ? row_bytes * 2 : row_bytes, static_cast<uint64_t>(rows), row_bytes, 128, static_cast<uint32_t>(box_rows),
+                                CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  auto scales_map = [&](CUtensorMap* map, uint64_t scales, int64_t rows) {
+    return encode_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, as_ptr<void>(scales), MX_TILE_BYTES / 4,
+                                static_cast<uint64_t>((rows + 127) / 128) * p.chunks, MX_TILE_BYTES, MX_TILE_BYTES / 4,
+                                static_cast<uint32_t>(scale_tiles), CU_TENSOR_MAP_SWIZZLE_NONE);
+  };
+  int rc;
+  if ((rc = codes_map(&maps[0], b_codes, format_b, p.N, spread_w, 128)) || (rc = codes_map(&maps[1], a_codes, format_a, p.M, spread_x, s.bt / s.ctas)) ||
+      (rc = scales_map(&maps[2], b_scales, p.N)) || (rc = scales_map(&maps[3], a_scales, p.M)))
+    return rc;
+  if (fp4) return s.ctas == 2 ? launch_mx<true, 2>(d, st, maps, p) : launch_mx<true, 1>(d, st, maps, p);
+  return s.ctas == 2 ? launch_mx<false, 2>(d, st, maps, p) : launch_mx<false, 1>(d, st, maps, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sb200_mx_bytes(int format, int64_t rows, int64_t K, uint64_t* codes, uint64_t* scales) {
+  if (int rc = check_format(format)) return rc;
+  if (int rc = check_shape(rows, K, "mx_bytes")) return rc;
+  if (!codes || !scales) return set_error(SB200_ERR_INVALID_VALUE, "mx_bytes: null result");
+  *codes = code_bytes(format, rows, K);
+  *scales = scale_bytes(rows, K);
+  return SB200_OK;
+}
+
+int sb200_mx_quantize(int dev, uint64_t stream, int format, int64_t rows, int64_t K, uint64_t src, int64_t ld, int transposed, uint64_t codes,
+                      uint64_t scales) {
+  OperatorDevice d;
+  if (int rc = operator_device(dev, &d)) return rc;
+  if (int rc = check_format(format)) return rc;
+  if (int rc = check_shape(rows, K, "mx_quantize")) return rc;
+  if (rows == 0 || K == 0) return SB200_OK;
+  if (int rc = check_matrix(dev, src, transposed ? K : rows, transposed ? rows : K, ld, "mx_quantize source")) return rc;
+  if (int rc = check_mx(dev, format, rows, K, codes, scales, "mx_quantize result")) return rc;
+  const MxQuantize q = {as_ptr<const float>(src), ld, rows, K, chunks_of(K), as_ptr<uint8_t>(codes), as_ptr<uint8_t>(scales)};
+  const cudaStream_t st = as_stream(stream);
+  const bool fp4 = format == SB200_MX_FP4;
+  if (transposed) {
+    const dim3 grid(grid_for((rows + 127) / 128 * 4 * ((q.chunks + 1) / 2), 1, 0x7fffffff));
+    CU_TRY(fp4 ? launch_pdl(mx_quantize_columns_kernel<true>, grid, dim3(256), 0, st, 1, q)
+               : launch_pdl(mx_quantize_columns_kernel<false>, grid, dim3(256), 0, st, 1, q));
+    return operator_launched("mx_quantize_columns_kernel");
+  }
+  const dim3 grid(grid_for((rows + 127) / 128 * 128 * q.chunks, 4 * (MX_QUANTIZE_THREADS / 32), 0x7fffffff)), block(MX_QUANTIZE_THREADS);
+  const bool vec = on_16(src, ld);
+  CU_TRY(fp4 ? (vec ? launch_pdl(mx_quantize_rows_kernel<true, true>, grid, block, 0, st, 1, q)
+                    : launch_pdl(mx_quantize_rows_kernel<true, false>, grid, block, 0, st, 1, q))
+             : (vec ? launch_pdl(mx_quantize_rows_kernel<false, true>, grid, block, 0, st, 1, q)
+                    : launch_pdl(mx_quantize_rows_kernel<false, false>, grid, block, 0, st, 1, q)));
+  return operator_launched("mx_quantize_rows_kernel");
+}
+
+int sb200_mx_dequantize(int dev, uint64_t stream, int format, int64_t rows, int64_t K, uint64_t codes, uint64_t scales, uint64_t dst, int64_t ld) {
+  OperatorDevice d;
+  if (int rc = operator_device(dev, &d)) return rc;
+  if (int rc = check_format(format)) return rc;
+  if (int rc = check_shape(rows, K, "mx_dequantize")) return rc;
+  if (rows == 0 || K == 0) return SB200_OK;
+  if (int rc = check_mx(dev, format, rows, K, codes, scales, "mx_dequantize operand")) return rc;
+  if (int rc = check_matrix(dev, dst, rows, K, ld, "mx_dequantize result")) return rc;
+  const MxDequantize q = {as_ptr<const uint8_t>(codes), as_ptr<const uint8_t>(scales), as_ptr<float>(dst), ld, rows, K, chunks_of(K)};
+  const cudaStream_t st = as_stream(stream);
+  const bool fp4 = format == SB200_MX_FP4, vec = on_16(dst, ld);
+  const dim3 grid(grid_for(rows * q.chunks, MX_QUANTIZE_THREADS / 32, static_cast<int64_t>(d.sm_count) * 64)), block(MX_QUANTIZE_THREADS);
+  CU_TRY(fp4 ? (vec ? launch_pdl(mx_dequantize_kernel<true, true>, grid, block, 0, st, 1, q)
+                    : launch_pdl(mx_dequantize_kernel<true, false>, grid, block, 0, st, 1, q))
+             : (vec ? launch_pdl(mx_dequantize_kernel<false, true>, grid, block, 0, st, 1, q)
+                    : launch_pdl(mx_dequantize_kernel<false, false>, grid, block, 0, st, 1, q)));
+  return operator_launched("mx_dequantize_kernel");
+}
+
+int sb200_gemm_mx(int dev, uint64_t stream, int format_a, int format_b, int64_t M, int64_t N, int64_t K, uint64_t a_codes, uint64_t a_scales,
+                  uint64_t b_codes, uint64_t b_scales, uint64_t D, int64_t ldd, float alpha, uint64_t C, int64_t ldc, float beta, uint64_t bias, int act) {
+  OperatorDevice d;
+  if (int rc = operator_device(dev, &d)) return rc;
+  if (int rc = check_format(format_a)) return rc;
+  if (int rc = check_format(format_b)) return rc;
+  if (int rc = check_shape(M, K, "gemm_mx")) return rc;
+  if (int rc = check_shape(N, K, "gemm_mx")) return rc;
+  if (act != SB200_ACT_NONE && act != SB200_ACT_RELU) return set_error(SB200_ERR_INVALID_VALUE, "unknown activation %d", act);
+  if (M == 0 || N == 0) return SB200_OK;
+  if (K > 0) {
+    if (int rc = check_mx(dev, format_a, M, K, a_codes, a_scales, "gemm_mx operand A")) return rc;
+    if (int rc = check_mx(dev, format_b, N, K, b_codes, b_scales, "gemm_mx operand B")) return rc;
+  }
+  if (int rc = check_matrix(dev, D, M, N, ldd, "gemm_mx result D")) return rc;
+  if (C)
+    if (int rc = check_matrix(dev, C, M, N, ldc, "gemm_mx operand C")) return rc;
+  if (bias)
+    if (int rc = check_matrix(dev, bias, 1, N, N, "gemm_mx bias")) return rc;
+  MxGemm p;
+  memset(&p, 0, sizeof p);
+  p.D = as_ptr<float>(D);
+  p.C = as_ptr<const float>(C);
+  p.bias = as_ptr<const float>(bias);
+  p.ldd = ldd;
+  p.ldc = ldc;
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.alpha = alpha;
+  p.beta = beta;
+  p.act = act;
+  if (K == 0) {
+    CU_TRY(launch_pdl(gemm_mx_empty_kernel, dim3(grid_for(M * N, 256, static_cast<int64_t>(d.sm_count) * 16)), dim3(256), 0, as_stream(stream), 1, p));
+    return operator_launched("gemm_mx_empty_kernel");
+  }
+  return run_gemm_mx(d, as_stream(stream), format_a, format_b, K, a_codes, a_scales, b_codes, b_scales, p);
+}
+
+int sb200_rmsnorm_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint64_t x, int64_t ldx, uint64_t residual, int64_t ldr, uint64_t weight,
+                      double eps, uint64_t sum, int64_t lds, uint64_t y, int64_t ldy, int format, uint64_t codes, uint64_t scales) {
+  OperatorDevice d;
+  if (int rc = operator_device(dev, &d)) return rc;
+  if (format != 0)
+    if (int rc = check_format(format)) return rc;
+  if (int rc = check_shape(rows, cols, "rmsnorm")) return rc;
+  if (!(eps >= 0.0)) return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm: eps must not be negative");
+  if (rows == 0 || cols == 0) return SB200_OK;
+  if (!sum && !y && format == 0) return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm: no result asked for");
+  if (int rc = check_matrix(dev, x, rows, cols, ldx, "rmsnorm x")) return rc;
+  if (int rc = check_matrix(dev, weight, 1, cols, cols, "rmsnorm weight")) return rc;
+  if (residual)
+    if (int rc = check_matrix(dev, residual, rows, cols, ldr, "rmsnorm residual")) return rc;
+  if (sum)
+    if (int rc = check_matrix(dev, sum, rows, cols, lds, "rmsnorm sum")) return rc;
+  if (y)
+    if (int rc = check_matrix(dev, y, rows, cols, ldy, "rmsnorm y")) return rc;
+  if (format)
+    if (int rc = check_mx(dev, format, rows, cols, codes, scales, "rmsnorm result")) return rc;
+  RmsNorm p;
+  memset(&p, 0, sizeof p);
+  p.x = as_ptr<const float>(x);
+  p.residual = as_ptr<const float>(residual);
+  p.weight = as_ptr<const float>(weight);
+  p.h = as_ptr<float>(sum);
+  p.y = as_ptr<float>(y);
+  p.ldx = ldx;
+  p.ldr = ldr;
+  p.ldh = lds;
+  p.ldy = ldy;
+  p.rows = rows;
+  p.cols = cols;
+  p.chunks = chunks_of(cols);
+  p.eps = eps;
+  if (format) {
+    p.codes = as_ptr<uint8_t>(codes);
+    p.scales = as_ptr<uint8_t>(scales);
+  }
+  // 128-bit accesses where every row of every matrix starts on 16 bytes
+  const bool vec = on_16(x, ldx) && on_16(weight, 0) && (!residual || on_16(residual, ldr)) && (!sum || on_16(sum, lds)) && (!y || on_16(y, ldy));
+  const cudaStream_t st = as_stream(stream);
+  if (format == SB200_MX_FP8) return vec ? launch_rmsnorm<8, true>(st, p) : launch_rmsnorm<8, false>(st, p);
+  if (format == SB200_MX_FP4) return vec ? launch_rmsnorm<4, true>(st, p) : launch_rmsnorm<4, false>(st, p);
+  return vec ? launch_rmsnorm<0, true>(st, p) : launch_rmsnorm<0, false>(st, p);
+}
+
+int sb200_rmsnorm_workspace_bytes(int64_t rows, int64_t cols, uint64_t* bytes) {
+  if (int rc = check_shape(rows, cols, "rmsnorm_workspace_bytes")) return rc;
+  if (!bytes) return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm_workspace_bytes: null result");
+  *bytes = static_cast<uint64_t>(dweight_parts(rows)) * cols * 4;
+  return SB200_OK;
+}
+
+int sb200_rmsnorm_backward_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint64_t sum, int64_t lds, uint64_t weight, double eps,
+                               uint64_t dy, int64_t lddy, uint64_t dsum, int64_t ldds, uint64_t dx, int64_t lddx, uint64_t dweight,
+                               uint64_t workspace, uint64_t workspace_bytes) {
+  OperatorDevice d;
+  if (int rc = operator_device(dev, &d)) return rc;
+  if (int rc = check_shape(rows, cols, "rmsnorm_backward")) return rc;
+  if (!(eps >= 0.0)) return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm_backward: eps must not be negative");
+  if (cols == 0) return SB200_OK;
+  if (!dx && !dweight) return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm_backward: no result asked for");
+  if (dweight)
+    if (int rc = check_matrix(dev, dweight, 1, cols, cols, "rmsnorm_backward dweight")) return rc;
+  const cudaStream_t st = as_stream(stream);
+  if (rows == 0) {  // an empty sum
+    if (dweight) CU_TRY(cudaMemsetAsync(as_ptr<void>(dweight), 0, static_cast<size_t>(cols) * 4, st));
+    return SB200_OK;
+  }
+  if (int rc = check_matrix(dev, sum, rows, cols, lds, "rmsnorm_backward sum")) return rc;
+  if (int rc = check_matrix(dev, weight, 1, cols, cols, "rmsnorm_backward weight")) return rc;
+  if (int rc = check_matrix(dev, dy, rows, cols, lddy, "rmsnorm_backward dy")) return rc;
+  if (dsum)
+    if (int rc = check_matrix(dev, dsum, rows, cols, ldds, "rmsnorm_backward dsum")) return rc;
+  if (dx)
+    if (int rc = check_matrix(dev, dx, rows, cols, lddx, "rmsnorm_backward dx")) return rc;
+  if (dweight) {
+    const uint64_t need = static_cast<uint64_t>(dweight_parts(rows)) * cols * 4;
+    if (!workspace || workspace_bytes < need)
+      return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm_backward: dweight needs a workspace of %llu bytes", static_cast<unsigned long long>(need));
+    if (workspace & 3) return set_error(SB200_ERR_ALIGNMENT, "rmsnorm_backward: the workspace must be 4-byte aligned");
+    if (int rc = operator_extent(dev, workspace, need, "rmsnorm_backward workspace")) return rc;
+  }
+  RmsNormBackward p;
+  memset(&p, 0, sizeof p);
+  p.h = as_ptr<const float>(sum);
+  p.weight = as_ptr<const float>(weight);
+  p.dy = as_ptr<const float>(dy);
+  p.dsum = as_ptr<const float>(dsum);
+  p.dx = as_ptr<float>(dx);
+  p.dweight = as_ptr<float>(dweight);
+  p.workspace = as_ptr<float>(workspace);
+  p.ldh = lds;
+  p.lddy = lddy;
+  p.ldds = ldds;
+  p.lddx = lddx;
+  p.rows = rows;
+  p.cols = cols;
+  p.eps = eps;
+  const bool vec = on_16(sum, lds) && on_16(weight, 0) && on_16(dy, lddy) && (!dsum || on_16(dsum, ldds)) && (!dx || on_16(dx, lddx));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(dweight_parts(rows), static_cast<int64_t>(d.sm_count) * 2));
+  return vec ? launch_rmsnorm_backward<true>(st, p, grid) : launch_rmsnorm_backward<false>(st, p, grid);
+}
+
+}  // extern "C"

@@ -221,29 +221,6 @@ int current_mode() {
   return m;
 }
 
-// Launches a kernel with programmatic stream serialization: it may set itself up while the kernel before it in the stream
-// still runs.  Every kernel launched this way passes griddepcontrol.wait before it touches global memory.  The launch call
-// itself is cheaper too (2.3 against 2.8 us).
-template <class... Params, class... Args>
-cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, Args&&... args) {
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof cfg);
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
-
 // --------------------------------------------------------------- map host
 template <class Op>
 int launch_map2(DeviceState& d, cudaStream_t st, const float* in0, const float* in1, float* out0, float* out1, float s,
@@ -2123,6 +2100,33 @@ int set_error(int code, const char* fmt, ...) {
   va_end(ap);
   g_err = buf;
   return code;
+}
+
+int set_cuda_error(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+
+int operator_device(int dev, OperatorDevice* out) {
+  DeviceState* d;
+  if (int rc = device_ready(dev, &d)) return rc;
+  out->index = dev;
+  out->sm_count = d->sm_count;
+  out->status = d->status;
+  return SB200_OK;
+}
+void operator_waits(int dev) { g_dev[dev].status_armed.store(true); }
+int operator_extent(int dev, uint64_t ptr, uint64_t bytes, const char* what) { return check_extent(g_dev[dev], ptr, bytes, what); }
+int operator_launched(const char* what) { return launch_check(what); }
+
+int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t rows, uint64_t row_bytes,
+                         uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  if (int rc = resolve_encode_tiled()) return rc;
+  const cuuint64_t dims[2] = {inner, rows}, strides[1] = {row_bytes};
+  const cuuint32_t box[2] = {box_inner, box_rows}, estr[2] = {1, 1};
+  const CUresult r = g_encode_tiled(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(SB200_ERR_INVALID_VALUE, "cuTensorMapEncodeTiled failed with CUresult %d (inner=%llu rows=%llu)", (int)r,
+                static_cast<unsigned long long>(inner), static_cast<unsigned long long>(rows));
+  return SB200_OK;
 }
 }  // namespace sb200
 
