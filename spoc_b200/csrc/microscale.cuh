@@ -63,31 +63,33 @@ __device__ __forceinline__ uint32_t largest_bits4(const float4& v) {  // bits of
   return max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)));
 }
 
-// A warp's chunk of a row: lane l has values 4l .. 4l + 3, eight lanes a block.  codes: of the chunk; scales: its four.
-template <bool FP4>
-__device__ __forceinline__ void mx_store_chunk(float4 v, uint8_t* codes, uint8_t* scales, int lane) {
+// A warp's chunk of a row: lane l has values 4l .. 4l + 3, eight lanes a block.
+__device__ __forceinline__ uint32_t largest_of_block(const float4& v) {
   uint32_t m = largest_bits4(v);
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-  const uint32_t scale = mx_scale_of<FP4>(m);
+  return max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+}
+// codes: of the chunk; scales: its four.
+template <bool FP4>
+__device__ __forceinline__ void mx_store_chunk(float4 v, uint32_t scale, uint8_t* codes, uint8_t* scales, int lane) {
   const uint32_t c = mx_codes4<FP4>(v, mx_factor(scale));
   if constexpr (FP4)
     reinterpret_cast<uint16_t*>(codes)[lane] = static_cast<uint16_t>(c);
   else
     reinterpret_cast<uint32_t*>(codes)[lane] = c;
-  uint32_t four = __shfl_sync(0xffffffffu, scale, 0);
-  four |= __shfl_sync(0xffffffffu, scale, 8) << 8;
-  four |= __shfl_sync(0xffffffffu, scale, 16) << 16;
-  four |= __shfl_sync(0xffffffffu, scale, 24) << 24;
-  if (lane == 0) *reinterpret_cast<uint32_t*>(scales) = four;
+  if ((lane & 7) == 0) scales[lane >> 3] = static_cast<uint8_t>(scale);
 }
 
-// Four values of a row from column `col` on; what is past `cols` counts for zero.  VEC: the row starts on 16 bytes.
+// Four values of a row from column `col` on; what is past `cols` counts for zero.  VEC: the row starts on 16 bytes and `cols` is a multiple of
+// four (the single elements beside the vectors cost the norm 30 registers a thread).
 template <bool VEC>
-__device__ __forceinline__ float4 load4(const float* row, long long col, long long cols) {
-  if (VEC && col + 4 <= cols) return *reinterpret_cast<const float4*>(row + col);
+__device__ __forceinline__ float4 load4(const float* row, int col, int cols) {
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (VEC) {
+    if (col < cols) v = *reinterpret_cast<const float4*>(row + col);
+    return v;
+  }
   if (col < cols) v.x = row[col];
   if (col + 1 < cols) v.y = row[col + 1];
   if (col + 2 < cols) v.z = row[col + 2];
@@ -95,9 +97,9 @@ __device__ __forceinline__ float4 load4(const float* row, long long col, long lo
   return v;
 }
 template <bool VEC>
-__device__ __forceinline__ void store4(float* row, long long col, long long cols, const float4& v) {
-  if (VEC && col + 4 <= cols) {
-    *reinterpret_cast<float4*>(row + col) = v;
+__device__ __forceinline__ void store4(float* row, int col, int cols, const float4& v) {
+  if (VEC) {
+    if (col < cols) *reinterpret_cast<float4*>(row + col) = v;
     return;
   }
   if (col < cols) row[col] = v.x;
@@ -136,13 +138,13 @@ __global__ void __launch_bounds__(MX_QUANTIZE_THREADS) mx_quantize_rows_kernel(c
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
-      v[u] = row[u] < q.rows ? load4<VEC>(q.src + row[u] * q.ld, chunk[u] * MX_CHUNK + 4 * lane, q.K) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[u] = row[u] < q.rows ? load4<VEC>(q.src + row[u] * q.ld, static_cast<int>(chunk[u]) * MX_CHUNK + 4 * lane, static_cast<int>(q.K)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       if (at + u >= all) break;
       uint8_t* scales = q.scales + mx_scale_offset(row[u], chunk[u], q.chunks);
       if (row[u] < q.rows)
-        mx_store_chunk<FP4>(v[u], q.codes + (row[u] * q.chunks + chunk[u]) * MxFormat<FP4>::kChunkBytes, scales, lane);
+        mx_store_chunk<FP4>(v[u], mx_scale_of<FP4>(largest_of_block(v[u])), q.codes + (row[u] * q.chunks + chunk[u]) * MxFormat<FP4>::kChunkBytes, scales, lane);
       else if (lane == 0)
         *reinterpret_cast<uint32_t*>(scales) = 0u;
     }
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(MX_QUANTIZE_THREADS) mx_dequantize_kernel(cons
       lo = __half22float2(__half2(a));
       hi = __half22float2(__half2(b));
     }
-    store4<VEC>(q.dst + row * q.ld, chunk * MX_CHUNK + 4 * lane, q.K, make_float4(lo.x * scale, lo.y * scale, hi.x * scale, hi.y * scale));
+    store4<VEC>(q.dst + row * q.ld, static_cast<int>(chunk) * MX_CHUNK + 4 * lane, static_cast<int>(q.K), make_float4(lo.x * scale, lo.y * scale, hi.x * scale, hi.y * scale));
   }
 }
 

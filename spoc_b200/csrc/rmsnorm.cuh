@@ -2,12 +2,15 @@
 //
 //   h = x + residual (rounded to float32: it is stored, and the next layer adds to it),  y = h * weight / sqrt(mean(h^2) + eps)
 //
-// y is computed in 64 bits from the h that is stored and rounded once.  A code of 8 or 4 bits is then the rounding of the exact y: next to a rounding
-// border 32 bits would fall on one side or the other depending on the order of the sum, one value in a million by a whole step, and so
-// would all that is computed from it.
+// A code of 8 or 4 bits is the rounding of the exact y of the stored h, with the sum of squares and the root in 64 bits: next to a rounding border
+// float32 falls on one side or the other depending on the order of the sum, one value in a million by a whole step, and so would all that is
+// computed from it.  64 bits throughout are not needed for that: y in float32 is at most seven units in the last place off (four from rsqrtf, two
+// products, the mean), and where a value of a warp's chunk lies within 16 of a border, or outside the range in which this holds, the warp does
+// the chunk over in 64 bits (rmsnorm_chunk_exact), one chunk of 250.
 //
-// One block a row, the row in registers (VECS float4 a thread; thread t has columns 4 (v * threads + t)), so that x and residual are read
-// once.  Rows too long for that (32768 columns on) are read twice.  Bound by HBM: 8 bytes read, 5 written a value with 8-bit codes.
+// A block a row, or a warp up to 1024 columns, the row in registers (VECS float4 a thread; thread t has columns 4 (v * threads + t)), so that x
+// and residual are read once.  Rows too long for that (32768 columns on) are read twice.  Bound by HBM: 8 bytes read, 5 written a value with
+// 8-bit codes, and by the blocks in flight: with 126 registers a thread there was one on an SM, and 8192 x 8192 took 337 us.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -21,8 +24,9 @@ struct RmsNorm {
   long long ldx, ldr, ldh, ldy;
   float *h, *y;                        // either may be null
   uint8_t *codes, *scales;             // null: no microscaled result
-  long long rows, cols, chunks;
-  double eps;
+  long long rows;
+  int cols, chunks;
+  double inv_cols, eps;
 };
 
 // Sum over the block of a value a thread, the same in all threads and in every launch.
@@ -49,23 +53,66 @@ __device__ __forceinline__ float round_to_odd(double y) {
   return __uint_as_float(b);
 }
 
-__device__ __forceinline__ double normed(float h, float w, double scale) { return static_cast<double>(h) * scale * static_cast<double>(w); }
+template <bool FP4>
+__device__ __noinline__ void rmsnorm_chunk_exact(float4 h, float4 w, double mean, uint8_t* codes, uint8_t* scales, int lane) {
+  const double scale = 1.0 / sqrt(mean);
+  const float4 y = make_float4(round_to_odd(h.x * scale * w.x), round_to_odd(h.y * scale * w.y), round_to_odd(h.z * scale * w.z),
+                               round_to_odd(h.w * scale * w.w));
+  mx_store_chunk<FP4>(y, mx_scale_of<FP4>(largest_of_block(y)), codes, scales, lane);
+}
 
-// What is done with four values of the normed row.  FORMAT: 0 float32 only, 4, 8.
+// Whether q, scaled for the type, lies so near the middle between two of its values that 16 units in the last place decide.  Below the type's
+// smallest normal value (2^-6, 1) the values are as far apart as right above it: moved there, all middles are the same pattern of the bits
+// that the rounding drops.
+template <bool FP4>
+__device__ __forceinline__ bool near_middle(float q) {
+  constexpr uint32_t DROPPED = FP4 ? 22 : 20;
+  const float smallest = FP4 ? 1.0f : 0.015625f, a = fabsf(q), v = a < smallest ? a + smallest : a;
+  return ((__float_as_uint(v) + 16u - (1u << (DROPPED - 1))) & ((1u << DROPPED) - 1u)) <= 32u;
+}
+
+// What a row's results need.
+struct RmsRow {
+  double mean;      // of the squares, plus eps
+  float scale;      // 1 / sqrt(mean), nearly
+  float* y;         // each result's row, or null
+  uint8_t *codes, *scales;
+};
+template <int FORMAT>
+__device__ __forceinline__ RmsRow rmsnorm_row(const RmsNorm& p, long long row, double sum) {
+  RmsRow r;
+  r.mean = fma(sum, p.inv_cols, p.eps);
+  r.scale = rsqrtf(static_cast<float>(r.mean));
+  r.y = p.y ? p.y + row * p.ldy : nullptr;
+  r.codes = p.codes + row * p.chunks * (FORMAT == 4 ? 64 : 128);
+  r.scales = p.scales + mx_scale_offset(row, 0, p.chunks);
+  return r;
+}
+// Four values of the normed row from column `col` on.  FORMAT: 0 float32 only, 4, 8.
 template <int FORMAT, bool VEC>
-__device__ __forceinline__ void rmsnorm_emit(const RmsNorm& p, long long row, long long col, const float4& h, double scale, int lane) {
-  float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (col < p.cols) w = load4<VEC>(p.weight, col, p.cols);
-  const double y[4] = {normed(h.x, w.x, scale), normed(h.y, w.y, scale), normed(h.z, w.z, scale), normed(h.w, w.w, scale)};
-  if (p.y)
-    store4<VEC>(p.y + row * p.ldy, col, p.cols,
-                make_float4(static_cast<float>(y[0]), static_cast<float>(y[1]), static_cast<float>(y[2]), static_cast<float>(y[3])));
+__device__ __forceinline__ void rmsnorm_emit(const RmsNorm& p, const RmsRow& row, int col, const float4& h, int lane) {
+  const float s = row.scale;
+  const float4 w = load4<VEC>(p.weight, col, p.cols);
+  const float4 y = make_float4(h.x * s * w.x, h.y * s * w.y, h.z * s * w.z, h.w * s * w.w);
+  if (row.y) store4<VEC>(row.y, col, p.cols, y);
   if constexpr (FORMAT != 0) {
     constexpr bool FP4 = FORMAT == 4;
-    const long long chunk = col / MX_CHUNK;  // the same in a whole warp
-    if (chunk < p.chunks)
-      mx_store_chunk<FP4>(make_float4(round_to_odd(y[0]), round_to_odd(y[1]), round_to_odd(y[2]), round_to_odd(y[3])),
-                          p.codes + (row * p.chunks + chunk) * MxFormat<FP4>::kChunkBytes, p.scales + mx_scale_offset(row, chunk, p.chunks), lane);
+    const int chunk = col / MX_CHUNK;  // the same in a whole warp
+    if (chunk >= p.chunks) return;
+    uint8_t* codes = row.codes + static_cast<long long>(chunk) * MxFormat<FP4>::kChunkBytes;
+    uint8_t* scales = row.scales + static_cast<long long>(chunk) * MX_TILE_BYTES;
+    const uint32_t m = largest_of_block(y), block_scale = mx_scale_of<FP4>(m);
+    const float f = mx_factor(block_scale);
+    // The estimate holds for weights below 2^40 and a largest value between 2^-60 and 2^100: products that fall below float32's range then lose
+    // nothing that a code shows.  A block of zeros holds too, where h is zero.
+    bool again = near_middle<FP4>(y.x * f) || near_middle<FP4>(y.y * f) || near_middle<FP4>(y.z * f) || near_middle<FP4>(y.w * f);
+    again = again || !(fmaxf(fmaxf(fabsf(w.x), fabsf(w.y)), fmaxf(fabsf(w.z), fabsf(w.w))) < 1.09951163e12f);
+    again = again || (m == 0 ? (abs_bits(h.x) | abs_bits(h.y) | abs_bits(h.z) | abs_bits(h.w)) != 0
+                             : m - (67u << 23) >= 160u << 23 || ((m + 16u) & 0x7fffffu) <= 32u);  // next to a power of two the scale is in question
+    if (__any_sync(0xffffffffu, again))
+      rmsnorm_chunk_exact<FP4>(h, w, row.mean, codes, scales, lane);
+    else
+      mx_store_chunk<FP4>(y, block_scale, codes, scales, lane);
   }
 }
 __device__ __forceinline__ double squares(const float4& h) {
@@ -73,7 +120,7 @@ __device__ __forceinline__ double squares(const float4& h) {
          fma(static_cast<double>(h.z), static_cast<double>(h.z), static_cast<double>(h.w) * h.w);
 }
 template <bool VEC>
-__device__ __forceinline__ float4 rmsnorm_input(const RmsNorm& p, long long row, long long col) {
+__device__ __forceinline__ float4 rmsnorm_input(const RmsNorm& p, long long row, int col) {
   float4 h = load4<VEC>(p.x + row * p.ldx, col, p.cols);
   if (p.residual) {
     const float4 r = load4<VEC>(p.residual + row * p.ldr, col, p.cols);
@@ -81,53 +128,49 @@ __device__ __forceinline__ float4 rmsnorm_input(const RmsNorm& p, long long row,
   }
   return h;
 }
-// VECS = 0: rows of any length, read twice (h may be x or residual itself: then the second reading takes h, which was stored).
-template <int FORMAT, int THREADS, int VECS, bool VEC>
-__global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const RmsNorm p) {
+// THREADS: of a row; 32: a block has four rows.  VECS = 0: rows of any length, read twice (h may be x or residual itself: then the second
+// reading takes h, which was stored).
+template <int FORMAT, int THREADS, int VECS, bool VEC, int BLOCKS>
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS, BLOCKS) rmsnorm_kernel(const RmsNorm p) {
+  constexpr int ROWS = THREADS == 32 ? 4 : 1;
   __shared__ double shared[2][THREADS / 32];
   grid_launch_dependents();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, thread = THREADS == 32 ? lane : threadIdx.x, first = 4 * thread;
   const long long rows = FORMAT ? (p.rows + 127) / 128 * 128 : p.rows;
   int turn = 0;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+  for (long long row = blockIdx.x * static_cast<long long>(ROWS) + (ROWS > 1 ? threadIdx.x >> 5 : 0); row < rows;
+       row += gridDim.x * static_cast<long long>(ROWS), turn ^= 1) {
     if (FORMAT && row >= p.rows) {  // the scales' padding
-      for (long long c = threadIdx.x; c < p.chunks; c += THREADS) *reinterpret_cast<uint32_t*>(p.scales + mx_scale_offset(row, c, p.chunks)) = 0u;
+      for (int c = thread; c < p.chunks; c += THREADS) *reinterpret_cast<uint32_t*>(p.scales + mx_scale_offset(row, c, p.chunks)) = 0u;
       continue;
     }
     if constexpr (VECS > 0) {
       float4 h[VECS];
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) h[v] = rmsnorm_input<VEC>(p, row, 4ll * (v * THREADS + threadIdx.x));
+      for (int v = 0; v < VECS; ++v) h[v] = rmsnorm_input<VEC>(p, row, first + v * 4 * THREADS);
       double s = 0.0;
 #pragma unroll
       for (int v = 0; v < VECS; ++v) s += squares(h[v]);
       if (p.h) {
+        float* to = p.h + row * p.ldh;
 #pragma unroll
-        for (int v = 0; v < VECS; ++v) store4<VEC>(p.h + row * p.ldh, 4ll * (v * THREADS + threadIdx.x), p.cols, h[v]);
+        for (int v = 0; v < VECS; ++v) store4<VEC>(to, first + v * 4 * THREADS, p.cols, h[v]);
       }
-      const double scale = 1.0 / sqrt(block_sum<THREADS>(s, shared[turn]) / static_cast<double>(p.cols) + p.eps);
+      const RmsRow r = rmsnorm_row<FORMAT>(p, row, block_sum<THREADS>(s, shared[turn]));
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) rmsnorm_emit<FORMAT, VEC>(p, row, 4ll * (v * THREADS + threadIdx.x), h[v], scale, lane);
+      for (int v = 0; v < VECS; ++v) rmsnorm_emit<FORMAT, VEC>(p, r, first + v * 4 * THREADS, h[v], lane);
     } else {
-      const long long padded = (p.cols + MX_CHUNK - 1) / MX_CHUNK * MX_CHUNK;
       double s = 0.0;
-      for (long long col = 4ll * threadIdx.x; col < p.cols; col += 4 * THREADS) {
-        const float4 h = rmsnorm_input<VEC>(p, row, col);
+      for (long long col = first; col < p.cols; col += 4 * THREADS) {
+        const float4 h = rmsnorm_input<VEC>(p, row, static_cast<int>(col));
         s += squares(h);
-        if (p.h) store4<VEC>(p.h + row * p.ldh, col, p.cols, h);
+        if (p.h) store4<VEC>(p.h + row * p.ldh, static_cast<int>(col), p.cols, h);
       }
-      const double scale = 1.0 / sqrt(block_sum<THREADS>(s, shared[turn]) / static_cast<double>(p.cols) + p.eps);
-      for (long long col = 4ll * threadIdx.x; col < padded; col += 4 * THREADS) {
-        float4 h;
-        if (p.h) {  // this thread's own stores; not through the read-only path
-          const float* src = p.h + row * p.ldh;
-          h = make_float4(col < p.cols ? src[col] : 0.f, col + 1 < p.cols ? src[col + 1] : 0.f, col + 2 < p.cols ? src[col + 2] : 0.f,
-                          col + 3 < p.cols ? src[col + 3] : 0.f);
-        } else {
-          h = rmsnorm_input<VEC>(p, row, col);
-        }
-        rmsnorm_emit<FORMAT, VEC>(p, row, col, h, scale, lane);
+      const RmsRow r = rmsnorm_row<FORMAT>(p, row, block_sum<THREADS>(s, shared[turn]));
+      for (long long col = first; col < static_cast<long long>(p.chunks) * MX_CHUNK; col += 4 * THREADS) {
+        const float4 h = p.h ? load4<VEC>(p.h + row * p.ldh, static_cast<int>(col), p.cols) : rmsnorm_input<VEC>(p, row, static_cast<int>(col));
+        rmsnorm_emit<FORMAT, VEC>(p, r, static_cast<int>(col), h, lane);
       }
     }
   }
@@ -141,7 +184,8 @@ struct RmsNormBackward {
   const float *h, *weight, *dy, *dsum;  // dsum may be null
   long long ldh, lddy, ldds, lddx;
   float *dx, *dweight, *workspace;      // either of dx and dweight may be null
-  long long rows, cols;
+  long long rows;
+  int cols;
   double eps;
 };
 template <int THREADS, int VECS, bool VEC>
@@ -149,12 +193,13 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
   __shared__ float2 shared[2][THREADS / 32];
   grid_launch_dependents();
   grid_dependency_wait();
+  const int first = 4 * threadIdx.x;
   const float inv_cols = 1.0f / static_cast<float>(p.cols), eps = static_cast<float>(p.eps);
   constexpr int HELD = VECS > 0 ? VECS : 1;
   float4 part[HELD];
 #pragma unroll
   for (int v = 0; v < HELD; ++v) part[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float* const mine = p.workspace + blockIdx.x * p.cols;
+  float* const mine = p.workspace + static_cast<long long>(blockIdx.x) * p.cols;
   int turn = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
     const float *hr = p.h + row * p.ldh, *dyr = p.dy + row * p.lddy;
@@ -167,14 +212,16 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
     if constexpr (VECS > 0) {
 #pragma unroll
       for (int v = 0; v < VECS; ++v) {
-        h[v] = load4<VEC>(hr, 4ll * (v * THREADS + threadIdx.x), p.cols);
-        dy[v] = load4<VEC>(dyr, 4ll * (v * THREADS + threadIdx.x), p.cols);
+        h[v] = load4<VEC>(hr, first + v * 4 * THREADS, p.cols);
+        dy[v] = load4<VEC>(dyr, first + v * 4 * THREADS, p.cols);
       }
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) count(h[v], dy[v], load4<VEC>(p.weight, 4ll * (v * THREADS + threadIdx.x), p.cols));
+      for (int v = 0; v < VECS; ++v) count(h[v], dy[v], load4<VEC>(p.weight, first + v * 4 * THREADS, p.cols));
     } else {
-      for (long long col = 4ll * threadIdx.x; col < p.cols; col += 4 * THREADS)
+      for (long long c = first; c < p.cols; c += 4 * THREADS) {
+        const int col = static_cast<int>(c);
         count(load4<VEC>(hr, col, p.cols), load4<VEC>(dyr, col, p.cols), load4<VEC>(p.weight, col, p.cols));
+      }
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -191,7 +238,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
     }
     const float r = 1.0f / sqrtf(s.x * inv_cols + eps);
     const float along = s.y * inv_cols * r * r;  // mean(g n) r: what h is multiplied by
-    auto finish = [&](long long col, const float4& a, const float4& d, float4& w_part) {
+    auto finish = [&](int col, const float4& a, const float4& d, float4& w_part) {
       if (p.dx) {
         const float4 w = load4<VEC>(p.weight, col, p.cols);
         float4 o = make_float4(r * fmaf(-a.x, along, d.x * w.x), r * fmaf(-a.y, along, d.y * w.y), r * fmaf(-a.z, along, d.z * w.z),
@@ -209,9 +256,10 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
     };
     if constexpr (VECS > 0) {
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) finish(4ll * (v * THREADS + threadIdx.x), h[v], dy[v], part[v]);
+      for (int v = 0; v < VECS; ++v) finish(first + v * 4 * THREADS, h[v], dy[v], part[v]);
     } else {
-      for (long long col = 4ll * threadIdx.x; col < p.cols; col += 4 * THREADS) {
+      for (long long c = first; c < p.cols; c += 4 * THREADS) {
+        const int col = static_cast<int>(c);
         float4 w_part = make_float4(0.f, 0.f, 0.f, 0.f);
         if (p.dweight && row != blockIdx.x)
           w_part = make_float4(mine[col], col + 1 < p.cols ? mine[col + 1] : 0.f, col + 2 < p.cols ? mine[col + 2] : 0.f,
@@ -225,7 +273,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
   if constexpr (VECS > 0) {
     if (p.dweight) {
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) store4<false>(mine, 4ll * (v * THREADS + threadIdx.x), p.cols, part[v]);
+      for (int v = 0; v < VECS; ++v) store4<false>(mine, first + v * 4 * THREADS, p.cols, part[v]);
     }
   }
 }

@@ -78,18 +78,21 @@ unsigned grid_for(int64_t work, int64_t per_block, int64_t cap) {
 template <int FORMAT, bool VEC>
 int launch_rmsnorm(cudaStream_t st, const RmsNorm& p) {
   const int64_t rows = FORMAT ? (p.rows + 127) / 128 * 128 : p.rows;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(rows, 0x7fffffff));
-  // the fewest float4 a thread that hold the row, in blocks of up to 1024 threads
-#define SB200_NORM(THREADS, VECS) CU_TRY(launch_pdl(rmsnorm_kernel<FORMAT, THREADS, VECS, VEC>, dim3(grid), dim3(THREADS), 0, st, 1, p))
-  const int64_t cols = p.cols;
-  if (cols <= 512) SB200_NORM(128, 1);
-  else if (cols <= 1024) SB200_NORM(256, 1);
-  else if (cols <= 2048) SB200_NORM(256, 2);
-  else if (cols <= 4096) SB200_NORM(256, 4);
-  else if (cols <= 8192) SB200_NORM(512, 4);
-  else if (cols <= 16384) SB200_NORM(512, 8);
-  else if (cols <= 32768) SB200_NORM(1024, 8);
-  else SB200_NORM(1024, 0);
+  // the row in the registers of a warp or a block, and as many blocks an SM as leave a thread 40 registers (64 with eight float4)
+#define SB200_NORM(THREADS, VECS, BLOCKS)                                                                                           \
+  CU_TRY(launch_pdl(rmsnorm_kernel<FORMAT, THREADS, VECS, VEC, BLOCKS>, dim3(grid_for(rows, THREADS == 32 ? 4 : 1, 0x7fffffff)),    \
+                    dim3(THREADS == 32 ? 128 : THREADS), 0, st, 1, p))
+  const int cols = p.cols;
+  if (cols <= 128) SB200_NORM(32, 1, 12);
+  else if (cols <= 256) SB200_NORM(32, 2, 12);
+  else if (cols <= 512) SB200_NORM(32, 4, 12);
+  else if (cols <= 1024) SB200_NORM(32, 8, 8);
+  else if (cols <= 2048) SB200_NORM(128, 4, 12);
+  else if (cols <= 4096) SB200_NORM(256, 4, 6);
+  else if (cols <= 8192) SB200_NORM(512, 4, 3);
+  else if (cols <= 16384) SB200_NORM(512, 8, 2);
+  else if (cols <= 32768) SB200_NORM(1024, 8, 1);
+  else SB200_NORM(1024, 0, 1);
 #undef SB200_NORM
   return operator_launched("rmsnorm_kernel");
 }
@@ -231,7 +234,7 @@ int sb200_mx_quantize(int dev, uint64_t stream, int format, int64_t rows, int64_
     return operator_launched("mx_quantize_columns_kernel");
   }
   const dim3 grid(grid_for((rows + 127) / 128 * 128 * q.chunks, 4 * (MX_QUANTIZE_THREADS / 32), 0x7fffffff)), block(MX_QUANTIZE_THREADS);
-  const bool vec = on_16(src, ld);
+  const bool vec = on_16(src, ld) && K % 4 == 0;
   CU_TRY(fp4 ? (vec ? launch_pdl(mx_quantize_rows_kernel<true, true>, grid, block, 0, st, 1, q)
                     : launch_pdl(mx_quantize_rows_kernel<true, false>, grid, block, 0, st, 1, q))
              : (vec ? launch_pdl(mx_quantize_rows_kernel<false, true>, grid, block, 0, st, 1, q)
@@ -249,7 +252,7 @@ int sb200_mx_dequantize(int dev, uint64_t stream, int format, int64_t rows, int6
   if (int rc = check_matrix(dev, dst, rows, K, ld, "mx_dequantize result")) return rc;
   const MxDequantize q = {as_ptr<const uint8_t>(codes), as_ptr<const uint8_t>(scales), as_ptr<float>(dst), ld, rows, K, chunks_of(K)};
   const cudaStream_t st = as_stream(stream);
-  const bool fp4 = format == SB200_MX_FP4, vec = on_16(dst, ld);
+  const bool fp4 = format == SB200_MX_FP4, vec = on_16(dst, ld) && K % 4 == 0;
   const dim3 grid(grid_for(rows * q.chunks, MX_QUANTIZE_THREADS / 32, static_cast<int64_t>(d.sm_count) * 64)), block(MX_QUANTIZE_THREADS);
   CU_TRY(fp4 ? (vec ? launch_pdl(mx_dequantize_kernel<true, true>, grid, block, 0, st, 1, q)
                     : launch_pdl(mx_dequantize_kernel<true, false>, grid, block, 0, st, 1, q))
@@ -328,15 +331,16 @@ int sb200_rmsnorm_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint
   p.ldh = lds;
   p.ldy = ldy;
   p.rows = rows;
-  p.cols = cols;
-  p.chunks = chunks_of(cols);
+  p.cols = static_cast<int>(cols);
+  p.chunks = static_cast<int>(chunks_of(cols));
+  p.inv_cols = 1.0 / static_cast<double>(cols);
   p.eps = eps;
   if (format) {
     p.codes = as_ptr<uint8_t>(codes);
     p.scales = as_ptr<uint8_t>(scales);
   }
-  // 128-bit accesses where every row of every matrix starts on 16 bytes
-  const bool vec = on_16(x, ldx) && on_16(weight, 0) && (!residual || on_16(residual, ldr)) && (!sum || on_16(sum, lds)) && (!y || on_16(y, ldy));
+  // 128-bit accesses where every row of every matrix starts on 16 bytes and has whole vectors
+  const bool vec = cols % 4 == 0 && on_16(x, ldx) && on_16(weight, 0) && (!residual || on_16(residual, ldr)) && (!sum || on_16(sum, lds)) && (!y || on_16(y, ldy));
   const cudaStream_t st = as_stream(stream);
   if (format == SB200_MX_FP8) return vec ? launch_rmsnorm<8, true>(st, p) : launch_rmsnorm<8, false>(st, p);
   if (format == SB200_MX_FP4) return vec ? launch_rmsnorm<4, true>(st, p) : launch_rmsnorm<4, false>(st, p);
@@ -394,9 +398,9 @@ int sb200_rmsnorm_backward_f32(int dev, uint64_t stream, int64_t rows, int64_t c
   p.ldds = ldds;
   p.lddx = lddx;
   p.rows = rows;
-  p.cols = cols;
+  p.cols = static_cast<int>(cols);
   p.eps = eps;
-  const bool vec = on_16(sum, lds) && on_16(weight, 0) && on_16(dy, lddy) && (!dsum || on_16(dsum, ldds)) && (!dx || on_16(dx, lddx));
+  const bool vec = cols % 4 == 0 && on_16(sum, lds) && on_16(weight, 0) && on_16(dy, lddy) && (!dsum || on_16(dsum, ldds)) && (!dx || on_16(dx, lddx));
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(dweight_parts(rows), static_cast<int64_t>(d.sm_count) * 2));
   return vec ? launch_rmsnorm_backward<true>(st, p, grid) : launch_rmsnorm_backward<false>(st, p, grid);
 }
