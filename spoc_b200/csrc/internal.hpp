@@ -52,6 +52,13 @@ cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t 
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Clusters of `blocks` (at most 8) blocks that are resident at once when every block has an SM to itself.  A cluster lies within a
+// GPC, whose SMs it may not divide evenly: the runtime counts 148, 74, 45, 33, 26, 22, 15 and 15 on a 148-SM B200.  One less from
+// three blocks on, because chips differ in the SMs that are switched off and one cluster too many is a second wave.
+inline long long cluster_capacity(int blocks, int sm_count) {
+  static const int resident[9] = {0, 148, 74, 44, 32, 25, 21, 14, 14};
+  return static_cast<long long>(resident[blocks]) * sm_count / 148;
+}
 // The numeric modes every GEMM entry point takes.
 inline bool valid_mode(int mode) {
   return mode == SB200_MODE_3XTF32 || mode == SB200_MODE_TF32 || mode == SB200_MODE_3XF16 || mode == SB200_MODE_F16 ||

@@ -124,36 +124,53 @@ struct MxShape {
 };
 int64_t mx_tiles(const MxShape& s, int64_t M, int64_t N) { return (N + 128 * s.ctas - 1) / (128 * s.ctas) * ((M + s.bt - 1) / s.bt); }
 
+// The shape with the least estimated time.  Measured on one B200, operands from L2 and HBM, in us: a launch with one k-block 3.3; a k-block 0.165 and
+// 0.4 ns a row of A in a block's tile (4 loads, 4 MMAs and a round of barriers, whatever the width up to 64 rows), half as much again where all
+// SMs load at once (128 x 2048 x 16384 0.21, 2048 x 4096 x 4096 0.29); in pairs 0.22 to 0.28 for 128 rows and 0.31 to 0.42 for 256; the last
+// epilogue 6 ns a row; a k-loop divided within a cluster 1.1 and 30 ns for every row a block sends (1 x 4096 x 4096 8.6 -> 5.7 us in four,
+// 64 x 4096 x 4096 9.3 -> 7.3).
 MxShape choose_mx_shape(int64_t M, int64_t N, int64_t k_blocks, int sm_count) {
-  MxShape s;
-  if (M <= 128) {
-    s.bt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  } else {
-    s.ctas = 2;
-    s.bt = 256;
-    if (mx_tiles(s, M, N) < sm_count / 2) s.bt = 128;
-    if (mx_tiles(s, M, N) < sm_count / 2) s.ctas = 1;
-  }
-  if (s.ctas == 1) {
-    const int64_t tiles = mx_tiles(s, M, N);
-    while (s.splits < 8 && tiles * s.splits * 2 <= sm_count && k_blocks >= s.splits * 4) s.splits *= 2;
-  }
-  return s;
+  MxShape best;
+  double best_us = 0.0;
+  auto consider = [&](int ctas, int bt, int splits) {
+    MxShape s;
+    s.ctas = ctas;
+    s.bt = bt;
+    s.splits = splits;
+    const int64_t tiles = mx_tiles(s, M, N), units = std::max(1, sm_count / ctas);
+    if (splits > 1 && tiles > cluster_capacity(splits, sm_count)) return;  // all clusters at once
+    const int64_t per_item = (k_blocks + splits - 1) / splits, waves = splits > 1 ? 1 : (tiles + units - 1) / units;
+    const double busy = std::min(1.0, static_cast<double>(tiles) * splits / units);
+    const double k_block = ctas == 1 ? (0.165 + 0.0004 * bt) * (bt == 128 ? 1.0 + 0.4 * busy : 1.0) : bt == 256 ? 0.31 + 0.11 * busy : 0.19 + 0.0003 * bt + 0.06 * busy;
+    double us = 3.3 + static_cast<double>(waves * per_item) * k_block + 0.006 * bt + 0.5 * static_cast<double>(waves - 1);
+    if (splits > 1) us += 1.1 + 0.03 * bt * (splits - 1) / splits;
+    if (best_us == 0.0 || us < 0.97 * best_us) {
+      best = s;
+      best_us = us;
+    }
+  };
+  const int narrow = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  for (int splits = 1; splits <= MXG_MAX_SPLITS; ++splits)
+    if (k_blocks >= 2 * splits || splits == 1) consider(1, narrow, splits);
+  if (narrow >= 64) consider(2, narrow, 1);
+  if (M > 128) consider(2, 256, 1);
+  return best;
 }
 
-template <bool FP4, int CTAS>
-int launch_mx(const OperatorDevice& d, cudaStream_t st, const CUtensorMap (&maps)[4], const MxGemm& p) {
-  auto kernel = gemm_mx_kernel<FP4, CTAS>;
-  constexpr int kSmem = 1024 + MXG_CTRL_BYTES + MXG_RING_BYTES;
+template <bool FP4, int CTAS, int GROUPS, bool IN_CLUSTER = false>
+int launch_mx(const OperatorDevice& d, cudaStream_t st, const CUtensorMap (&maps)[6], const MxGemm& p) {
+  auto kernel = gemm_mx_kernel<FP4, CTAS, GROUPS, IN_CLUSTER>;
+  constexpr int kMost = 1024 + MXG_CTRL_BYTES + MXG_RING_BYTES;
+  const int smem = 1024 + MXG_CTRL_BYTES + std::max(p.stages * p.stage_bytes, IN_CLUSTER ? p.bt * 512 : 0);
   static std::atomic<bool> ready[kMaxDevices];
   if (!ready[d.index].load()) {
-    CU_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    CU_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
     ready[d.index].store(true);
   }
   const int tiles = p.tiles_f * p.tiles_t, units = d.sm_count / CTAS;
   const int grid = p.splits > 1 ? tiles * p.splits : CTAS * std::min(tiles, units);
   operator_waits(d.index);
-  CU_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(MXG_THREADS), kSmem, st, CTAS * p.splits, maps[0], maps[1], maps[2], maps[3], p));
+  CU_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(MXG_THREADS), smem, st, CTAS * p.splits, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p));
   return operator_launched("gemm_mx_kernel");
 }
 
@@ -168,21 +185,37 @@ int run_gemm_mx(const OperatorDevice& d, cudaStream_t st, int format_a, int form
   p.bt = s.bt;
   p.tiles_f = static_cast<int>((p.N + 128ll * s.ctas - 1) / (128 * s.ctas));
   p.tiles_t = static_cast<int>((p.M + static_cast<int64_t>(s.bt) - 1) / s.bt);
-  p.groups = s.bt > 128 ? 2 : 1;
+  const int groups = s.bt > 128 ? 2 : 1;  // tiles of 128 rows of A's scales that a tile touches
   p.split_k_blocks = (p.num_k_blocks + s.splits - 1) / s.splits;
   p.splits = (p.num_k_blocks + p.split_k_blocks - 1) / p.split_k_blocks;  // the last one has something to do
   const int scale_tiles = fp4 ? 2 : 1;
-  const int x_bytes = s.bt / s.ctas * 128, sf_bytes = scale_tiles * MX_TILE_BYTES * (1 + p.groups);
+  const int x_bytes = s.bt / s.ctas * 128, sf_bytes = scale_tiles * MX_TILE_BYTES * (1 + groups);
   p.stage_bytes = (static_cast<int>(MXG_W_BYTES) + x_bytes + sf_bytes + 1023) / 1024 * 1024;
   p.stages = std::min(MXG_MAX_STAGES, MXG_RING_BYTES / p.stage_bytes);
-  p.accs = 2 * s.bt + 2 * 4 * scale_tiles * (1 + p.groups) <= MXG_TMEM_COLS ? 2 : 1;
+  const int sf_cols = 4 * scale_tiles * (1 + groups), units = d.sm_count / s.ctas;
+  if (tiles <= units || p.splits > 1) {
+    // A tile a block: no more stages than k-blocks, one accumulator, and no more tensor memory than that takes, so that the blocks of the
+    // launch behind this one can set themselves up beside these.
+    p.stages = std::max(1, std::min(p.stages, p.split_k_blocks));
+    const int held = std::max(32, s.bt);
+    p.slots = std::min(p.stages, (MXG_TMEM_COLS - held) / sf_cols);
+    p.tmem_cols = 32;
+    while (p.tmem_cols < held + p.slots * sf_cols) p.tmem_cols *= 2;
+    p.acc1 = s.bt;
+  } else {
+    // two accumulators, which overlap by 64 columns at most
+    p.slots = std::min(p.stages, (MXG_TMEM_COLS - 2 * s.bt + (s.bt == 256 ? 64 : 0)) / sf_cols);
+    p.tmem_cols = MXG_TMEM_COLS;
+    p.acc1 = std::min(256, MXG_TMEM_COLS - p.slots * sf_cols - s.bt);
+  }
   // spread: 4-bit codes that TMA spreads to a byte a value; a barrier counts the bytes that it reads
   const bool spread_w = !fp4 && format_b == SB200_MX_FP4, spread_x = !fp4 && format_a == SB200_MX_FP4;
-  p.tx_bytes = s.ctas * ((static_cast<int>(MXG_W_BYTES) >> (spread_w ? 1 : 0)) + (x_bytes >> (spread_x ? 1 : 0)) + sf_bytes);
+  p.w_row_bytes = spread_w ? 64 : 128;
+  p.x_row_bytes = spread_x ? 64 : 128;
   p.idesc = umma_idesc_mx(128u * s.ctas, static_cast<uint32_t>(s.bt), fp4 ? 1u : format_b == SB200_MX_FP4 ? 5u : 0u,
                           fp4 ? 1u : format_a == SB200_MX_FP4 ? 5u : 0u);
   p.status = d.status;
-  CUtensorMap maps[4];
+  CUtensorMap maps[6];
   auto codes_map = [&](CUtensorMap* map, uint64_t codes, int format, int64_t rows, bool spread, int box_rows) {
     const uint64_t row_bytes = static_cast<uint64_t>(p.chunks) * (format == SB200_MX_FP4 ? 64 : 128);
     return encode_tensor_map_2d(map, spread ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, as_ptr<void>(codes),
@@ -194,12 +227,22 @@ int run_gemm_mx(const OperatorDevice& d, cudaStream_t st, int format_a, int form
                                 static_cast<uint64_t>((rows + 127) / 128) * p.chunks, MX_TILE_BYTES, MX_TILE_BYTES / 4,
                                 static_cast<uint32_t>(scale_tiles), CU_TENSOR_MAP_SWIZZLE_NONE);
   };
+  const int part_t = s.bt / s.ctas;
+  const int w_tail = p.N % 128 ? p.N % 128 : 128, x_tail = p.M % part_t ? p.M % part_t : part_t;
+  p.w_tail = w_tail;
+  p.x_tail = x_tail;
   int rc;
-  if ((rc = codes_map(&maps[0], b_codes, format_b, p.N, spread_w, 128)) || (rc = codes_map(&maps[1], a_codes, format_a, p.M, spread_x, s.bt / s.ctas)) ||
-      (rc = scales_map(&maps[2], b_scales, p.N)) || (rc = scales_map(&maps[3], a_scales, p.M)))
+  if ((rc = codes_map(&maps[0], b_codes, format_b, p.N, spread_w, 128)) || (rc = codes_map(&maps[1], a_codes, format_a, p.M, spread_x, part_t)) ||
+      (w_tail < 128 && (rc = codes_map(&maps[2], b_codes, format_b, p.N, spread_w, w_tail))) ||
+      (x_tail < part_t && (rc = codes_map(&maps[3], a_codes, format_a, p.M, spread_x, x_tail))) || (rc = scales_map(&maps[4], b_scales, p.N)) ||
+      (rc = scales_map(&maps[5], a_scales, p.M)))
     return rc;
-  if (fp4) return s.ctas == 2 ? launch_mx<true, 2>(d, st, maps, p) : launch_mx<true, 1>(d, st, maps, p);
-  return s.ctas == 2 ? launch_mx<false, 2>(d, st, maps, p) : launch_mx<false, 1>(d, st, maps, p);
+  if (w_tail == 128) maps[2] = maps[0];
+  if (x_tail == part_t) maps[3] = maps[1];
+  if (p.splits > 1) return fp4 ? launch_mx<true, 1, 1, true>(d, st, maps, p) : launch_mx<false, 1, 1, true>(d, st, maps, p);
+  if (s.ctas == 1) return fp4 ? launch_mx<true, 1, 1>(d, st, maps, p) : launch_mx<false, 1, 1>(d, st, maps, p);
+  if (groups == 1) return fp4 ? launch_mx<true, 2, 1>(d, st, maps, p) : launch_mx<false, 2, 1>(d, st, maps, p);
+  return fp4 ? launch_mx<true, 2, 2>(d, st, maps, p) : launch_mx<false, 2, 2>(d, st, maps, p);
 }
 
 }  // namespace

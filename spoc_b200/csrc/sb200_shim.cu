@@ -487,13 +487,6 @@ struct TileShape {
   double cost = 0.0;  // estimated time, ns
 };
 
-// Clusters of `blocks` (at most 8) blocks that are resident at once when every block has an SM to itself.  A cluster lies within a
-// GPC, whose SMs it may not divide evenly: the runtime counts 148, 74, 45, 33, 26, 22, 15 and 15 on a 148-SM B200.  One less from
-// three blocks on, because chips differ in the SMs that are switched off and one cluster too many is a second wave.
-long long cluster_capacity(int blocks, int sm_count) {
-  static const int resident[9] = {0, 148, 74, 44, 32, 25, 21, 14, 14};
-  return static_cast<long long>(resident[blocks]) * sm_count / 148;
-}
 // Whether the items of a divided k-loop are the blocks (pairs) of one cluster: at most eight blocks, the portable size, and
 // all tiles at once, because a cluster works on one tile and ends.
 bool split_in_cluster(long long tiles, int splits, int ctas, int sm_count) {
