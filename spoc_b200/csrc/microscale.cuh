@@ -115,99 +115,113 @@ struct MxQuantize {
 };
 constexpr int MX_QUANTIZE_THREADS = 256;
 
-// Rows of a matrix: a warp a chunk, MX_AHEAD chunks in flight.  Bound by HBM: 4 bytes read, 1 (1/2) and 1/32 written a value.
+// A warp's work in the kernels over rows: up to MX_AHEAD chunks side by side in one row, so that one division finds them (32 bits wide where the
+// number of warps allows it: 64 bits take 100 instructions, as much as all else).
+constexpr int MX_AHEAD = 4;
+struct MxWarp {
+  long long row;
+  int chunk;
+};
+__device__ __forceinline__ MxWarp mx_warp(long long chunks, long long warps) {
+  const long long at = static_cast<long long>(blockIdx.x) * (MX_QUANTIZE_THREADS / 32) + (threadIdx.x >> 5), groups = (chunks + MX_AHEAD - 1) / MX_AHEAD;
+  MxWarp w;
+  if (warps < (1ll << 31)) {
+    const unsigned int row = static_cast<unsigned int>(at) / static_cast<unsigned int>(groups);
+    w.row = row;
+    w.chunk = static_cast<int>(static_cast<unsigned int>(at) - row * static_cast<unsigned int>(groups)) * MX_AHEAD;
+  } else {
+    w.row = at / groups;
+    w.chunk = static_cast<int>(at - w.row * groups) * MX_AHEAD;
+  }
+  return w;
+}
+
+// Rows of a matrix.  Bound by HBM: 4 bytes read, 1 (1/2) and 1/32 written a value.
 template <bool FP4, bool VEC>
-__global__ void __launch_bounds__(MX_QUANTIZE_THREADS) mx_quantize_rows_kernel(const MxQuantize q) {
-  constexpr int AHEAD = 4;
+__global__ void __launch_bounds__(MX_QUANTIZE_THREADS) mx_quantize_rows_kernel(const MxQuantize q, long long warps) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const long long warps = static_cast<long long>(gridDim.x) * (MX_QUANTIZE_THREADS / 32);
-  const long long first = static_cast<long long>(blockIdx.x) * (MX_QUANTIZE_THREADS / 32) + (threadIdx.x >> 5);
-  const long long all = (q.rows + 127) / 128 * 128 * q.chunks;
-  for (long long at = first * AHEAD; at < all; at += warps * AHEAD) {
-    float4 v[AHEAD];
-    long long row[AHEAD], chunk[AHEAD];
-    row[0] = at / q.chunks;
-    chunk[0] = at - row[0] * q.chunks;
+  const int lane = threadIdx.x & 31, cols = static_cast<int>(q.K), chunks = static_cast<int>(q.chunks);
+  const MxWarp w = mx_warp(q.chunks, warps);
+  if (w.row >= (q.rows + 127) / 128 * 128) return;
+  uint8_t* scales = q.scales + mx_scale_offset(w.row, w.chunk, q.chunks);
+  if (w.row >= q.rows) {
+    if (lane < MX_AHEAD && w.chunk + lane < chunks) *reinterpret_cast<uint32_t*>(scales + lane * MX_TILE_BYTES) = 0u;
+    return;
+  }
+  const float* src = q.src + w.row * q.ld;
+  uint8_t* codes = q.codes + (w.row * q.chunks + w.chunk) * MxFormat<FP4>::kChunkBytes;
+  float4 v[MX_AHEAD];
 #pragma unroll
-    for (int u = 1; u < AHEAD; ++u) {
-      const bool next = chunk[u - 1] + 1 == q.chunks;
-      row[u] = row[u - 1] + (next ? 1 : 0);
-      chunk[u] = next ? 0 : chunk[u - 1] + 1;
-    }
+  for (int u = 0; u < MX_AHEAD; ++u) v[u] = load4<VEC>(src, min(w.chunk + u, chunks) * MX_CHUNK + 4 * lane, cols);
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-      v[u] = row[u] < q.rows ? load4<VEC>(q.src + row[u] * q.ld, static_cast<int>(chunk[u]) * MX_CHUNK + 4 * lane, static_cast<int>(q.K)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      if (at + u >= all) break;
-      uint8_t* scales = q.scales + mx_scale_offset(row[u], chunk[u], q.chunks);
-      if (row[u] < q.rows)
-        mx_store_chunk<FP4>(v[u], mx_scale_of<FP4>(largest_of_block(v[u])), q.codes + (row[u] * q.chunks + chunk[u]) * MxFormat<FP4>::kChunkBytes, scales, lane);
-      else if (lane == 0)
-        *reinterpret_cast<uint32_t*>(scales) = 0u;
-    }
+  for (int u = 0; u < MX_AHEAD; ++u) {
+    if (w.chunk + u >= chunks) break;
+    mx_store_chunk<FP4>(v[u], mx_scale_of<FP4>(largest_of_block(v[u])), codes + u * MxFormat<FP4>::kChunkBytes, scales + u * MX_TILE_BYTES, lane);
   }
 }
 
-// Columns of a matrix stored K x rows: a block takes 32 of its columns (rows of the result) and 256 of its rows, a thread 32 values below one
+// Columns of a matrix stored K x rows: a block takes 64 of its columns (rows of the result) and 256 of its rows, a thread 32 values below one
 // another, which is a block with one scale.  The codes go through shared memory, so that a row's 256 (128) bytes are written together.
+// Bound by HBM as the kernel over rows is.
+constexpr int MX_COLUMNS = 64;
+constexpr int MX_COLUMNS_THREADS = 8 * MX_COLUMNS;
 template <bool FP4>
-__global__ void __launch_bounds__(256) mx_quantize_columns_kernel(const MxQuantize q) {
+__global__ void __launch_bounds__(MX_COLUMNS_THREADS) mx_quantize_columns_kernel(const MxQuantize q) {
   constexpr int BYTES = FP4 ? 16 : 32;            // codes of a block
   constexpr int PITCH = 8 * BYTES + 16;           // 16 more: rows start on different banks
-  __shared__ __align__(16) uint8_t codes[32 * PITCH];
-  __shared__ uint8_t scales[32][8];
+  __shared__ __align__(16) uint8_t codes[MX_COLUMNS * PITCH];
+  __shared__ __align__(8) uint8_t scales[MX_COLUMNS][8];
   grid_launch_dependents();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long row_tiles = (q.rows + 127) / 128 * 4, k_tiles = (q.chunks + 1) / 2;
-  const long long tiles = row_tiles * k_tiles;
-  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const long long kt = tile / row_tiles, row0 = (tile - kt * row_tiles) * 32;
-    const long long k0 = kt * 256 + warp * 32;
-    float v[32];
-    const float* src = q.src + k0 * q.ld + row0 + lane;
-    const bool in = row0 + lane < q.rows;
+  const int column = threadIdx.x % MX_COLUMNS, block = threadIdx.x / MX_COLUMNS;
+  const unsigned int row_tiles = static_cast<unsigned int>((q.rows + 127) / 128) * (128 / MX_COLUMNS), kt = blockIdx.x / row_tiles;
+  const long long row0 = static_cast<long long>(blockIdx.x - kt * row_tiles) * MX_COLUMNS;
+  const long long k0 = kt * 256ll + block * 32;
+  float v[32];
+  const float* src = q.src + k0 * q.ld + row0 + column;
+  if (row0 + column < q.rows && k0 + 32 <= q.K) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = in && k0 + i < q.K ? __ldg(src + i * q.ld) : 0.0f;
-    uint32_t m = 0;
+    for (int i = 0; i < 32; ++i) v[i] = src[i * q.ld];
+  } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) m = max(m, abs_bits(v[i]));
-    const uint32_t scale = mx_scale_of<FP4>(m);
-    const float factor = mx_factor(scale);
-    uint32_t words[BYTES / 4];
+    for (int i = 0; i < 32; ++i) v[i] = row0 + column < q.rows && k0 + i < q.K ? src[i * q.ld] : 0.0f;
+  }
+  uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t c = mx_codes4<FP4>(make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]), factor);
-      if constexpr (FP4)
-        words[i / 2] = i % 2 ? words[i / 2] | c << 16 : c;
-      else
-        words[i] = c;
+  for (int i = 0; i < 32; ++i) m = max(m, abs_bits(v[i]));
+  const uint32_t scale = mx_scale_of<FP4>(m);
+  const float factor = mx_factor(scale);
+  uint32_t words[BYTES / 4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t c = mx_codes4<FP4>(make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]), factor);
+    if constexpr (FP4)
+      words[i / 2] = i % 2 ? words[i / 2] | c << 16 : c;
+    else
+      words[i] = c;
+  }
+  uint8_t* to = codes + column * PITCH + block * BYTES;
+#pragma unroll
+  for (int i = 0; i < BYTES / 16; ++i)
+    reinterpret_cast<uint4*>(to)[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+  scales[column][block] = static_cast<uint8_t>(scale);
+  __syncthreads();
+  constexpr int QUADS = 8 * BYTES / 16;  // 16-byte pieces of a row
+  const int chunks = static_cast<int>(min(2ll, q.chunks - kt * 2ll)), pieces = chunks * (QUADS / 2);
+#pragma unroll
+  for (int i = threadIdx.x; i < MX_COLUMNS * QUADS; i += MX_COLUMNS_THREADS) {
+    const int r = i / QUADS, piece = i % QUADS;
+    if (row0 + r < q.rows && piece < pieces)
+      *reinterpret_cast<uint4*>(q.codes + ((row0 + r) * q.chunks + kt * 2ll) * MxFormat<FP4>::kChunkBytes + piece * 16) =
+          *reinterpret_cast<const uint4*>(codes + r * PITCH + piece * 16);
+  }
+  if (threadIdx.x < 2 * MX_COLUMNS) {
+    const int r = threadIdx.x >> 1, half = threadIdx.x & 1;
+    if (half < chunks) {
+      const uint32_t four = *reinterpret_cast<const uint32_t*>(&scales[r][half * 4]);
+      *reinterpret_cast<uint32_t*>(q.scales + mx_scale_offset(row0 + r, kt * 2ll + half, q.chunks)) = row0 + r < q.rows ? four : 0u;
     }
-    uint8_t* to = codes + lane * PITCH + warp * BYTES;
-#pragma unroll
-    for (int i = 0; i < BYTES / 16; ++i)
-      reinterpret_cast<uint4*>(to)[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
-    scales[lane][warp] = static_cast<uint8_t>(scale);
-    __syncthreads();
-    constexpr int QUADS = 8 * BYTES / 16;  // 16-byte pieces of a row
-    const int pieces = static_cast<int>(min(2ll, q.chunks - kt * 2)) * (QUADS / 2);
-    for (int i = threadIdx.x; i < 32 * QUADS; i += 256) {
-      const int r = i / QUADS, piece = i % QUADS;
-      if (row0 + r < q.rows && piece < pieces)
-        *reinterpret_cast<uint4*>(q.codes + ((row0 + r) * q.chunks + kt * 2) * MxFormat<FP4>::kChunkBytes + piece * 16) =
-            *reinterpret_cast<const uint4*>(codes + r * PITCH + piece * 16);
-    }
-    if (threadIdx.x < 64) {
-      const int r = threadIdx.x >> 1, half = threadIdx.x & 1;
-      if (kt * 2 + half < q.chunks) {
-        const uint32_t four = *reinterpret_cast<const uint32_t*>(&scales[r][half * 4]);
-        *reinterpret_cast<uint32_t*>(q.scales + mx_scale_offset(row0 + r, kt * 2 + half, q.chunks)) = row0 + r < q.rows ? four : 0u;
-      }
-    }
-    __syncthreads();
   }
 }
 
@@ -218,30 +232,38 @@ struct MxDequantize {
   long long ld, rows, K, chunks;
 };
 template <bool FP4, bool VEC>
-__global__ void __launch_bounds__(MX_QUANTIZE_THREADS) mx_dequantize_kernel(const MxDequantize q) {
+__global__ void __launch_bounds__(MX_QUANTIZE_THREADS) mx_dequantize_kernel(const MxDequantize q, long long warps) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const long long warps = static_cast<long long>(gridDim.x) * (MX_QUANTIZE_THREADS / 32);
-  for (long long at = static_cast<long long>(blockIdx.x) * (MX_QUANTIZE_THREADS / 32) + (threadIdx.x >> 5); at < q.rows * q.chunks; at += warps) {
-    const long long row = at / q.chunks, chunk = at - row * q.chunks;
-    const uint8_t* codes = q.codes + at * MxFormat<FP4>::kChunkBytes;
-    const float scale = mx_scale_value(q.scales[mx_scale_offset(row, chunk, q.chunks) + lane / 8]);
-    float2 lo, hi;
+  const int lane = threadIdx.x & 31, chunks = static_cast<int>(q.chunks);
+  const MxWarp w = mx_warp(q.chunks, warps);
+  if (w.row >= q.rows) return;
+  const uint8_t* codes = q.codes + (w.row * q.chunks + w.chunk) * MxFormat<FP4>::kChunkBytes;
+  const uint8_t* scales = q.scales + mx_scale_offset(w.row, w.chunk, q.chunks) + lane / 8;
+  uint32_t c[MX_AHEAD], scale[MX_AHEAD];
+#pragma unroll
+  for (int u = 0; u < MX_AHEAD; ++u) {
+    const int at = min(u, chunks - 1 - w.chunk);
+    if constexpr (FP4)
+      c[u] = reinterpret_cast<const uint16_t*>(codes + at * MxFormat<FP4>::kChunkBytes)[lane];
+    else
+      c[u] = reinterpret_cast<const uint32_t*>(codes + at * MxFormat<FP4>::kChunkBytes)[lane];
+    scale[u] = scales[at * MX_TILE_BYTES];
+  }
+#pragma unroll
+  for (int u = 0; u < MX_AHEAD; ++u) {
+    if (w.chunk + u >= chunks) break;
+    __half2_raw a, b;
     if constexpr (FP4) {
-      const uint32_t c = reinterpret_cast<const uint16_t*>(codes)[lane];
-      const __half2_raw a = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(c & 255u), __NV_E2M1);
-      const __half2_raw b = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(c >> 8), __NV_E2M1);
-      lo = __half22float2(__half2(a));
-      hi = __half22float2(__half2(b));
+      a = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(c[u] & 255u), __NV_E2M1);
+      b = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(c[u] >> 8), __NV_E2M1);
     } else {
-      const uint32_t c = reinterpret_cast<const uint32_t*>(codes)[lane];
-      const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c & 65535u), __NV_E4M3);
-      const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c >> 16), __NV_E4M3);
-      lo = __half22float2(__half2(a));
-      hi = __half22float2(__half2(b));
+      a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c[u] & 65535u), __NV_E4M3);
+      b = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c[u] >> 16), __NV_E4M3);
     }
-    store4<VEC>(q.dst + row * q.ld, static_cast<int>(chunk) * MX_CHUNK + 4 * lane, static_cast<int>(q.K), make_float4(lo.x * scale, lo.y * scale, hi.x * scale, hi.y * scale));
+    const float2 lo = __half22float2(__half2(a)), hi = __half22float2(__half2(b));
+    const float f = mx_scale_value(scale[u]);
+    store4<VEC>(q.dst + w.row * q.ld, (w.chunk + u) * MX_CHUNK + 4 * lane, static_cast<int>(q.K), make_float4(lo.x * f, lo.y * f, hi.x * f, hi.y * f));
   }
 }
 

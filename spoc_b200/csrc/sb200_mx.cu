@@ -271,17 +271,18 @@ int sb200_mx_quantize(int dev, uint64_t stream, int format, int64_t rows, int64_
   const cudaStream_t st = as_stream(stream);
   const bool fp4 = format == SB200_MX_FP4;
   if (transposed) {
-    const dim3 grid(grid_for((rows + 127) / 128 * 4 * ((q.chunks + 1) / 2), 1, 0x7fffffff));
-    CU_TRY(fp4 ? launch_pdl(mx_quantize_columns_kernel<true>, grid, dim3(256), 0, st, 1, q)
-               : launch_pdl(mx_quantize_columns_kernel<false>, grid, dim3(256), 0, st, 1, q));
+    const dim3 grid(grid_for((rows + 127) / 128 * (128 / MX_COLUMNS) * ((q.chunks + 1) / 2), 1, 0x7fffffff)), block(MX_COLUMNS_THREADS);
+    CU_TRY(fp4 ? launch_pdl(mx_quantize_columns_kernel<true>, grid, block, 0, st, 1, q)
+               : launch_pdl(mx_quantize_columns_kernel<false>, grid, block, 0, st, 1, q));
     return operator_launched("mx_quantize_columns_kernel");
   }
-  const dim3 grid(grid_for((rows + 127) / 128 * 128 * q.chunks, 4 * (MX_QUANTIZE_THREADS / 32), 0x7fffffff)), block(MX_QUANTIZE_THREADS);
+  const long long warps = (rows + 127) / 128 * 128 * ((q.chunks + MX_AHEAD - 1) / MX_AHEAD);
+  const dim3 grid(grid_for(warps, MX_QUANTIZE_THREADS / 32, 0x7fffffff)), block(MX_QUANTIZE_THREADS);
   const bool vec = on_16(src, ld) && K % 4 == 0;
-  CU_TRY(fp4 ? (vec ? launch_pdl(mx_quantize_rows_kernel<true, true>, grid, block, 0, st, 1, q)
-                    : launch_pdl(mx_quantize_rows_kernel<true, false>, grid, block, 0, st, 1, q))
-             : (vec ? launch_pdl(mx_quantize_rows_kernel<false, true>, grid, block, 0, st, 1, q)
-                    : launch_pdl(mx_quantize_rows_kernel<false, false>, grid, block, 0, st, 1, q)));
+  CU_TRY(fp4 ? (vec ? launch_pdl(mx_quantize_rows_kernel<true, true>, grid, block, 0, st, 1, q, warps)
+                    : launch_pdl(mx_quantize_rows_kernel<true, false>, grid, block, 0, st, 1, q, warps))
+             : (vec ? launch_pdl(mx_quantize_rows_kernel<false, true>, grid, block, 0, st, 1, q, warps)
+                    : launch_pdl(mx_quantize_rows_kernel<false, false>, grid, block, 0, st, 1, q, warps)));
   return operator_launched("mx_quantize_rows_kernel");
 }
 
@@ -296,11 +297,12 @@ int sb200_mx_dequantize(int dev, uint64_t stream, int format, int64_t rows, int6
   const MxDequantize q = {as_ptr<const uint8_t>(codes), as_ptr<const uint8_t>(scales), as_ptr<float>(dst), ld, rows, K, chunks_of(K)};
   const cudaStream_t st = as_stream(stream);
   const bool fp4 = format == SB200_MX_FP4, vec = on_16(dst, ld) && K % 4 == 0;
-  const dim3 grid(grid_for(rows * q.chunks, MX_QUANTIZE_THREADS / 32, static_cast<int64_t>(d.sm_count) * 64)), block(MX_QUANTIZE_THREADS);
-  CU_TRY(fp4 ? (vec ? launch_pdl(mx_dequantize_kernel<true, true>, grid, block, 0, st, 1, q)
-                    : launch_pdl(mx_dequantize_kernel<true, false>, grid, block, 0, st, 1, q))
-             : (vec ? launch_pdl(mx_dequantize_kernel<false, true>, grid, block, 0, st, 1, q)
-                    : launch_pdl(mx_dequantize_kernel<false, false>, grid, block, 0, st, 1, q)));
+  const long long warps = rows * ((q.chunks + MX_AHEAD - 1) / MX_AHEAD);
+  const dim3 grid(grid_for(warps, MX_QUANTIZE_THREADS / 32, 0x7fffffff)), block(MX_QUANTIZE_THREADS);
+  CU_TRY(fp4 ? (vec ? launch_pdl(mx_dequantize_kernel<true, true>, grid, block, 0, st, 1, q, warps)
+                    : launch_pdl(mx_dequantize_kernel<true, false>, grid, block, 0, st, 1, q, warps))
+             : (vec ? launch_pdl(mx_dequantize_kernel<false, true>, grid, block, 0, st, 1, q, warps)
+                    : launch_pdl(mx_dequantize_kernel<false, false>, grid, block, 0, st, 1, q, warps)));
   return operator_launched("mx_dequantize_kernel");
 }
 
