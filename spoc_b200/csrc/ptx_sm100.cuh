@@ -147,6 +147,11 @@ __device__ __forceinline__ void tma_load_2d_hint(uint32_t dst_smem, const CUtens
       ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "l"(policy)
       : "memory");
 }
+// Untiled bulk copy global -> this block's shared memory, completing its bytes on the mbarrier.  Addresses and size are multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(uint32_t dst_smem, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst_smem), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
 // 2-D tiled bulk-tensor store, this block's shared memory -> global; what lies outside the tensor is not written.
 // Completion is tracked per thread: bulk_commit() closes a group, bulk_wait_read<N>() returns once all but the last N
 // groups have read their shared memory.

@@ -184,6 +184,7 @@ struct RmsNormBackward {
   const float *h, *weight, *dy, *dsum;  // dsum may be null
   long long ldh, lddy, ldds, lddx;
   float *dx, *dweight, *workspace;      // either of dx and dweight may be null
+  int* status;
   long long rows;
   int cols;
   double eps;
@@ -277,6 +278,139 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
     }
   }
 }
+// The same for rows that TMA can copy (16-byte aligned, a multiple of four values) and a block's registers hold: groups of TG threads go from row to
+// row, each with a ring of STAGES rows of h, dy and dsum in shared memory that bulk copies fill ahead of it, so that the copies of one row run
+// under the sums of another (8192 x 4096: 131 us with a row's loads in front of its sums, see the table of times in the launch function).
+template <int TG, int G, int VECS, int STAGES>
+struct BackwardRing {
+  static constexpr int kThreads = TG * G, kCols = TG * VECS * 4;
+  static constexpr int kArrayBytes = kCols * 4, kStageBytes = 3 * kArrayBytes;
+  static constexpr int kBytes = G * STAGES * kStageBytes + 128;  // the copies start on 128 bytes
+  static_assert(G * kArrayBytes <= G * STAGES * kStageBytes, "the groups' parts of dweight fit the ring");
+};
+template <int TG, int G, int VECS, int STAGES, int BLOCKS>
+__global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(const RmsNormBackward p) {
+  using Ring = BackwardRing<TG, G, VECS, STAGES>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[G * STAGES];
+  __shared__ float2 sums[2][G * TG / 32];
+  __shared__ int abort_word;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  const int group = threadIdx.x / TG, thread = threadIdx.x % TG, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = 4 * thread;
+  uint8_t* mine = ring + group * STAGES * Ring::kStageBytes;
+  if (threadIdx.x < G * STAGES) {
+    mbar_init(smem_u32(&full[threadIdx.x]), 1);
+    mbar_fence_init();
+  }
+  if (threadIdx.x == 0) abort_word = 0;
+  __syncthreads();
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const float inv_cols = 1.0f / static_cast<float>(p.cols), eps = static_cast<float>(p.eps);
+  const long long step = static_cast<long long>(gridDim.x) * G, row0 = blockIdx.x * static_cast<long long>(G) + group;
+  const uint32_t bytes = static_cast<uint32_t>(p.cols) * 4;
+  auto fetch = [&](int stage, long long row) {  // one thread
+    const uint32_t bar = smem_u32(&full[group * STAGES + stage]), to = smem_u32(mine) + stage * Ring::kStageBytes;
+    mbar_arrive_expect_tx(bar, p.dsum ? 3 * bytes : 2 * bytes);
+    bulk_load(to, p.h + row * p.ldh, bytes, bar);
+    bulk_load(to + Ring::kArrayBytes, p.dy + row * p.lddy, bytes, bar);
+    if (p.dsum) bulk_load(to + 2 * Ring::kArrayBytes, p.dsum + row * p.ldds, bytes, bar);
+  };
+  if (thread == 0) {
+#pragma unroll 1
+    for (int s = 0; s < STAGES; ++s)
+      if (row0 + s * step < p.rows) fetch(s, row0 + s * step);
+  }
+  float4 w[VECS], part[VECS];
+#pragma unroll
+  for (int v = 0; v < VECS; ++v) {
+    w[v] = load4<true>(p.weight, first + v * 4 * TG, p.cols);
+    part[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (long long row = row0; row < p.rows; row += step, turn ^= 1) {
+    const uint8_t* from = mine + stage * Ring::kStageBytes;
+    ok = mbar_wait_bounded(smem_u32(&full[group * STAGES + stage]), phase, &abort_word);
+    float4 h[VECS], dy[VECS], ds[VECS];
+    float2 s = make_float2(0.f, 0.f);  // of h^2 and of h * g
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const int col = first + v * 4 * TG;
+      h[v] = dy[v] = ds[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (col < p.cols) {
+        h[v] = *reinterpret_cast<const float4*>(from + col * 4);
+        dy[v] = *reinterpret_cast<const float4*>(from + Ring::kArrayBytes + col * 4);
+        if (p.dsum) ds[v] = *reinterpret_cast<const float4*>(from + 2 * Ring::kArrayBytes + col * 4);
+      }
+      const float4 &a = h[v], &d = dy[v];
+      s.x += fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w);
+      s.y += fmaf(a.x, d.x * w[v].x, a.y * (d.y * w[v].y)) + fmaf(a.z, d.z * w[v].z, a.w * (d.w * w[v].w));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+      s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+    }
+    if (TG > 32) {
+      if (lane == 0) sums[turn][warp] = s;
+      ok = barrier_all(1 + group, TG, ok);  // the group has read the stage; all of it goes on, or none
+      s = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < TG / 32; ++k) {
+        s.x += sums[turn][group * (TG / 32) + k].x;
+        s.y += sums[turn][group * (TG / 32) + k].y;
+      }
+    } else {
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (!ok) break;
+    if (thread == 0 && row + STAGES * step < p.rows) fetch(stage, row + STAGES * step);
+    const float r = 1.0f / sqrtf(s.x * inv_cols + eps);
+    const float along = s.y * inv_cols * r * r;  // mean(g n) r: what h is multiplied by
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const float4 &a = h[v], &d = dy[v];
+      if (p.dx) {
+        const float4 o = make_float4(r * fmaf(-a.x, along, d.x * w[v].x) + ds[v].x, r * fmaf(-a.y, along, d.y * w[v].y) + ds[v].y,
+                                     r * fmaf(-a.z, along, d.z * w[v].z) + ds[v].z, r * fmaf(-a.w, along, d.w * w[v].w) + ds[v].w);
+        store4<true>(p.dx + row * p.lddx, first + v * 4 * TG, p.cols, o);
+      }
+      part[v].x = fmaf(d.x, a.x * r, part[v].x);
+      part[v].y = fmaf(d.y, a.y * r, part[v].y);
+      part[v].z = fmaf(d.z, a.z * r, part[v].z);
+      part[v].w = fmaf(d.w, a.w * r, part[v].w);
+    }
+    if (++stage == STAGES) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  if (!ok) {
+    if (lane == 0) atomicCAS(p.status, 0, 0x3100 | group);
+    wait_for_copies();
+  }
+  if (!p.dweight) return;
+  float* const to = p.workspace + static_cast<long long>(blockIdx.x) * p.cols;
+  if (G == 1) {
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) store4<false>(to, first + v * 4 * TG, p.cols, part[v]);
+    return;
+  }
+  __syncthreads();  // no copy is in flight: every group has waited for all that it asked for
+  float* const shared_part = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int v = 0; v < VECS; ++v) *reinterpret_cast<float4*>(shared_part + group * Ring::kCols + first + v * 4 * TG) = part[v];
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.cols; c += TG * G) {
+    float s = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) s += shared_part[g * Ring::kCols + c];
+    to[c] = s;
+  }
+}
+
 // dweight[c] = sum over the blocks of their parts: eight threads a column take every eighth part, whose sums are added in a fixed order.
 __global__ void __launch_bounds__(256) rmsnorm_dweight_kernel(const float* workspace, int parts, float* dweight, long long cols) {
   __shared__ float shared[8][32];

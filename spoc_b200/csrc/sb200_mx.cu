@@ -97,9 +97,35 @@ int launch_rmsnorm(cudaStream_t st, const RmsNorm& p) {
   return operator_launched("rmsnorm_kernel");
 }
 
+int64_t dweight_parts(int64_t rows) { return std::min<int64_t>(rows, SB200_RMSNORM_MAX_PARTS); }
+
+template <int TG, int G, int VECS, int STAGES, int BLOCKS>
+int launch_backward_ring(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, unsigned* grid) {
+  using Ring = BackwardRing<TG, G, VECS, STAGES>;
+  auto kernel = rmsnorm_backward_ring_kernel<TG, G, VECS, STAGES, BLOCKS>;
+  static std::atomic<bool> ready[kMaxDevices];
+  if (!ready[d.index].load()) {
+    CU_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring::kBytes));
+    ready[d.index].store(true);
+  }
+  *grid = static_cast<unsigned>(std::min<int64_t>((p.rows + G - 1) / G, std::min(d.sm_count * BLOCKS, SB200_RMSNORM_MAX_PARTS)));
+  operator_waits(d.index);
+  CU_TRY(launch_pdl(kernel, dim3(*grid), dim3(TG * G), Ring::kBytes, st, 1, p));
+  return operator_launched("rmsnorm_backward_ring_kernel");
+}
+int launch_backward_rings(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, unsigned* grid) {
+  const int cols = p.cols;
+  if (cols <= 128) return launch_backward_ring<32, 8, 1, 4, 3>(d, st, p, grid);
+  if (cols <= 512) return launch_backward_ring<128, 2, 1, 5, 3>(d, st, p, grid);
+  if (cols <= 1024) return launch_backward_ring<256, 1, 1, 5, 3>(d, st, p, grid);
+  if (cols <= 2048) return launch_backward_ring<256, 1, 2, 3, 3>(d, st, p, grid);
+  if (cols <= 4096) return launch_backward_ring<512, 1, 2, 2, 2>(d, st, p, grid);
+  return launch_backward_ring<1024, 1, 2, 2, 1>(d, st, p, grid);
+}
 template <bool VEC>
-int launch_rmsnorm_backward(cudaStream_t st, const RmsNormBackward& p, unsigned grid) {
-#define SB200_NORM(THREADS, VECS) CU_TRY(launch_pdl(rmsnorm_backward_kernel<THREADS, VECS, VEC>, dim3(grid), dim3(THREADS), 0, st, 1, p))
+int launch_backward_rows(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, unsigned* grid) {
+  *grid = static_cast<unsigned>(std::min<int64_t>(dweight_parts(p.rows), static_cast<int64_t>(d.sm_count) * 2));
+#define SB200_NORM(THREADS, VECS) CU_TRY(launch_pdl(rmsnorm_backward_kernel<THREADS, VECS, VEC>, dim3(*grid), dim3(THREADS), 0, st, 1, p))
   const int64_t cols = p.cols;
   if (cols <= 512) SB200_NORM(128, 1);
   else if (cols <= 1024) SB200_NORM(256, 1);
@@ -109,13 +135,18 @@ int launch_rmsnorm_backward(cudaStream_t st, const RmsNormBackward& p, unsigned 
   else if (cols <= 16384) SB200_NORM(512, 8);
   else SB200_NORM(1024, 0);
 #undef SB200_NORM
-  if (int rc = operator_launched("rmsnorm_backward_kernel")) return rc;
-  if (!p.dweight) return SB200_OK;
+  return operator_launched("rmsnorm_backward_kernel");
+}
+int launch_rmsnorm_backward(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, bool vec) {
+  unsigned grid = 0;
+  int rc;
+  if (vec && p.cols <= 8192) rc = launch_backward_rings(d, st, p, &grid);
+  else rc = vec ? launch_backward_rows<true>(d, st, p, &grid) : launch_backward_rows<false>(d, st, p, &grid);
+  if (rc || !p.dweight) return rc;
   CU_TRY(launch_pdl(rmsnorm_dweight_kernel, dim3(grid_for(p.cols, 32, 1 << 20)), dim3(256), 0, st, 1, static_cast<const float*>(p.workspace),
                     static_cast<int>(grid), p.dweight, static_cast<long long>(p.cols)));
   return operator_launched("rmsnorm_dweight_kernel");
 }
-int64_t dweight_parts(int64_t rows) { return std::min<int64_t>(rows, SB200_RMSNORM_MAX_PARTS); }
 
 // --------------------------------------------------------------- product
 // Tiles: 128 (256: pairs) columns of D by bt rows.
@@ -446,8 +477,8 @@ int sb200_rmsnorm_backward_f32(int dev, uint64_t stream, int64_t rows, int64_t c
   p.cols = static_cast<int>(cols);
   p.eps = eps;
   const bool vec = cols % 4 == 0 && on_16(sum, lds) && on_16(weight, 0) && on_16(dy, lddy) && (!dsum || on_16(dsum, ldds)) && (!dx || on_16(dx, lddx));
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(dweight_parts(rows), static_cast<int64_t>(d.sm_count) * 2));
-  return vec ? launch_rmsnorm_backward<true>(st, p, grid) : launch_rmsnorm_backward<false>(st, p, grid);
+  p.status = d.status;
+  return launch_rmsnorm_backward(d, st, p, vec);
 }
 
 }  // extern "C"
