@@ -52,20 +52,27 @@ int check_shape(int64_t rows, int64_t K, const char* what) {
 int check_format(int format) {
   return known_format(format) ? SB200_OK : set_error(SB200_ERR_INVALID_VALUE, "unknown microscaled format %d", format);
 }
-// A microscaled operand that is there: both buffers, where TMA can read them, inside their allocations.
-int check_mx(int dev, int format, int64_t rows, int64_t K, uint64_t codes, uint64_t scales, const char* what) {
+// A microscaled operand that is there: both buffers, where TMA can read them.
+int check_mx(uint64_t codes, uint64_t scales, const char* what) {
   if (!codes || !scales) return set_error(SB200_ERR_INVALID_VALUE, "%s: null codes or scales", what);
   if ((codes | scales) & 31) return set_error(SB200_ERR_ALIGNMENT, "%s: codes and scales start on 32 bytes", what);
-  if (int rc = operator_extent(dev, codes, code_bytes(format, rows, K), what)) return rc;
-  return operator_extent(dev, scales, scale_bytes(rows, K), what);
+  return SB200_OK;
 }
 // A float32 matrix that is there.
-int check_matrix(int dev, uint64_t p, int64_t rows, int64_t cols, int64_t ld, const char* what) {
+int check_matrix(uint64_t p, int64_t rows, int64_t cols, int64_t ld, const char* what) {
   if (!p) return set_error(SB200_ERR_INVALID_VALUE, "%s: null device pointer", what);
   if (p & 3) return set_error(SB200_ERR_ALIGNMENT, "%s: float32 matrices must be 4-byte aligned", what);
   if (ld < cols) return set_error(SB200_ERR_INVALID_VALUE, "%s: leading dimension %lld smaller than the row length %lld", what, (long long)ld, (long long)cols);
   if (ld > INT64_MAX / 8 / (rows > 0 ? rows : 1)) return set_error(SB200_ERR_TOO_LARGE, "%s: extent beyond 64 bits", what);
-  return rows && cols ? operator_extent(dev, p, (static_cast<uint64_t>(rows - 1) * ld + cols) * 4, what) : SB200_OK;
+  return SB200_OK;
+}
+// What lies in a buffer of the library's ends there.
+int mx_extent(int dev, int format, int64_t rows, int64_t K, uint64_t codes, uint64_t scales, const char* what) {
+  if (int rc = operator_extent(dev, codes, code_bytes(format, rows, K), what)) return rc;
+  return operator_extent(dev, scales, scale_bytes(rows, K), what);
+}
+int matrix_extent(int dev, uint64_t p, int64_t rows, int64_t cols, int64_t ld, const char* what) {
+  return p && rows && cols ? operator_extent(dev, p, (static_cast<uint64_t>(rows - 1) * ld + cols) * 4, what) : SB200_OK;
 }
 
 // Blocks for `work` units, `per_block` each, at most `waves` waves of what fits a chip.
@@ -291,13 +298,19 @@ int sb200_mx_bytes(int format, int64_t rows, int64_t K, uint64_t* codes, uint64_
 
 int sb200_mx_quantize(int dev, uint64_t stream, int format, int64_t rows, int64_t K, uint64_t src, int64_t ld, int transposed, uint64_t codes,
                       uint64_t scales) {
-  OperatorDevice d;
-  if (int rc = operator_device(dev, &d)) return rc;
   if (int rc = check_format(format)) return rc;
   if (int rc = check_shape(rows, K, "mx_quantize")) return rc;
-  if (rows == 0 || K == 0) return SB200_OK;
-  if (int rc = check_matrix(dev, src, transposed ? K : rows, transposed ? rows : K, ld, "mx_quantize source")) return rc;
-  if (int rc = check_mx(dev, format, rows, K, codes, scales, "mx_quantize result")) return rc;
+  const int64_t src_rows = transposed ? K : rows, src_cols = transposed ? rows : K;
+  const bool empty = rows == 0 || K == 0;
+  if (!empty) {
+    if (int rc = check_matrix(src, src_rows, src_cols, ld, "mx_quantize source")) return rc;
+    if (int rc = check_mx(codes, scales, "mx_quantize result")) return rc;
+  }
+  OperatorDevice d;
+  if (int rc = operator_device(dev, &d)) return rc;
+  if (empty) return SB200_OK;
+  if (int rc = matrix_extent(dev, src, src_rows, src_cols, ld, "mx_quantize source")) return rc;
+  if (int rc = mx_extent(dev, format, rows, K, codes, scales, "mx_quantize result")) return rc;
   const MxQuantize q = {as_ptr<const float>(src), ld, rows, K, chunks_of(K), as_ptr<uint8_t>(codes), as_ptr<uint8_t>(scales)};
   const cudaStream_t st = as_stream(stream);
   const bool fp4 = format == SB200_MX_FP4;
@@ -318,13 +331,18 @@ int sb200_mx_quantize(int dev, uint64_t stream, int format, int64_t rows, int64_
 }
 
 int sb200_mx_dequantize(int dev, uint64_t stream, int format, int64_t rows, int64_t K, uint64_t codes, uint64_t scales, uint64_t dst, int64_t ld) {
-  OperatorDevice d;
-  if (int rc = operator_device(dev, &d)) return rc;
   if (int rc = check_format(format)) return rc;
   if (int rc = check_shape(rows, K, "mx_dequantize")) return rc;
-  if (rows == 0 || K == 0) return SB200_OK;
-  if (int rc = check_mx(dev, format, rows, K, codes, scales, "mx_dequantize operand")) return rc;
-  if (int rc = check_matrix(dev, dst, rows, K, ld, "mx_dequantize result")) return rc;
+  const bool empty = rows == 0 || K == 0;
+  if (!empty) {
+    if (int rc = check_mx(codes, scales, "mx_dequantize operand")) return rc;
+    if (int rc = check_matrix(dst, rows, K, ld, "mx_dequantize result")) return rc;
+  }
+  OperatorDevice d;
+  if (int rc = operator_device(dev, &d)) return rc;
+  if (empty) return SB200_OK;
+  if (int rc = mx_extent(dev, format, rows, K, codes, scales, "mx_dequantize operand")) return rc;
+  if (int rc = matrix_extent(dev, dst, rows, K, ld, "mx_dequantize result")) return rc;
   const MxDequantize q = {as_ptr<const uint8_t>(codes), as_ptr<const uint8_t>(scales), as_ptr<float>(dst), ld, rows, K, chunks_of(K)};
   const cudaStream_t st = as_stream(stream);
   const bool fp4 = format == SB200_MX_FP4, vec = on_16(dst, ld) && K % 4 == 0;
@@ -339,23 +357,33 @@ int sb200_mx_dequantize(int dev, uint64_t stream, int format, int64_t rows, int6
 
 int sb200_gemm_mx(int dev, uint64_t stream, int format_a, int format_b, int64_t M, int64_t N, int64_t K, uint64_t a_codes, uint64_t a_scales,
                   uint64_t b_codes, uint64_t b_scales, uint64_t D, int64_t ldd, float alpha, uint64_t C, int64_t ldc, float beta, uint64_t bias, int act) {
-  OperatorDevice d;
-  if (int rc = operator_device(dev, &d)) return rc;
   if (int rc = check_format(format_a)) return rc;
   if (int rc = check_format(format_b)) return rc;
   if (int rc = check_shape(M, K, "gemm_mx")) return rc;
   if (int rc = check_shape(N, K, "gemm_mx")) return rc;
   if (act != SB200_ACT_NONE && act != SB200_ACT_RELU) return set_error(SB200_ERR_INVALID_VALUE, "unknown activation %d", act);
-  if (M == 0 || N == 0) return SB200_OK;
-  if (K > 0) {
-    if (int rc = check_mx(dev, format_a, M, K, a_codes, a_scales, "gemm_mx operand A")) return rc;
-    if (int rc = check_mx(dev, format_b, N, K, b_codes, b_scales, "gemm_mx operand B")) return rc;
+  const bool empty = M == 0 || N == 0;
+  if (!empty) {
+    if (K > 0) {
+      if (int rc = check_mx(a_codes, a_scales, "gemm_mx operand A")) return rc;
+      if (int rc = check_mx(b_codes, b_scales, "gemm_mx operand B")) return rc;
+    }
+    if (int rc = check_matrix(D, M, N, ldd, "gemm_mx result D")) return rc;
+    if (C)
+      if (int rc = check_matrix(C, M, N, ldc, "gemm_mx operand C")) return rc;
+    if (bias)
+      if (int rc = check_matrix(bias, 1, N, N, "gemm_mx bias")) return rc;
   }
-  if (int rc = check_matrix(dev, D, M, N, ldd, "gemm_mx result D")) return rc;
-  if (C)
-    if (int rc = check_matrix(dev, C, M, N, ldc, "gemm_mx operand C")) return rc;
-  if (bias)
-    if (int rc = check_matrix(dev, bias, 1, N, N, "gemm_mx bias")) return rc;
+  OperatorDevice d;
+  if (int rc = operator_device(dev, &d)) return rc;
+  if (empty) return SB200_OK;
+  if (K > 0) {
+    if (int rc = mx_extent(dev, format_a, M, K, a_codes, a_scales, "gemm_mx operand A")) return rc;
+    if (int rc = mx_extent(dev, format_b, N, K, b_codes, b_scales, "gemm_mx operand B")) return rc;
+  }
+  if (int rc = matrix_extent(dev, D, M, N, ldd, "gemm_mx result D")) return rc;
+  if (int rc = matrix_extent(dev, C, M, N, ldc, "gemm_mx operand C")) return rc;
+  if (int rc = matrix_extent(dev, bias, 1, N, N, "gemm_mx bias")) return rc;
   MxGemm p;
   memset(&p, 0, sizeof p);
   p.D = as_ptr<float>(D);
@@ -377,24 +405,34 @@ int sb200_gemm_mx(int dev, uint64_t stream, int format_a, int format_b, int64_t 
 
 int sb200_rmsnorm_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint64_t x, int64_t ldx, uint64_t residual, int64_t ldr, uint64_t weight,
                       double eps, uint64_t sum, int64_t lds, uint64_t y, int64_t ldy, int format, uint64_t codes, uint64_t scales) {
-  OperatorDevice d;
-  if (int rc = operator_device(dev, &d)) return rc;
   if (format != 0)
     if (int rc = check_format(format)) return rc;
   if (int rc = check_shape(rows, cols, "rmsnorm")) return rc;
   if (!(eps >= 0.0)) return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm: eps must not be negative");
-  if (rows == 0 || cols == 0) return SB200_OK;
   if (!sum && !y && format == 0) return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm: no result asked for");
-  if (int rc = check_matrix(dev, x, rows, cols, ldx, "rmsnorm x")) return rc;
-  if (int rc = check_matrix(dev, weight, 1, cols, cols, "rmsnorm weight")) return rc;
-  if (residual)
-    if (int rc = check_matrix(dev, residual, rows, cols, ldr, "rmsnorm residual")) return rc;
-  if (sum)
-    if (int rc = check_matrix(dev, sum, rows, cols, lds, "rmsnorm sum")) return rc;
-  if (y)
-    if (int rc = check_matrix(dev, y, rows, cols, ldy, "rmsnorm y")) return rc;
+  const bool empty = rows == 0 || cols == 0;
+  if (!empty) {
+    if (int rc = check_matrix(x, rows, cols, ldx, "rmsnorm x")) return rc;
+    if (int rc = check_matrix(weight, 1, cols, cols, "rmsnorm weight")) return rc;
+    if (residual)
+      if (int rc = check_matrix(residual, rows, cols, ldr, "rmsnorm residual")) return rc;
+    if (sum)
+      if (int rc = check_matrix(sum, rows, cols, lds, "rmsnorm sum")) return rc;
+    if (y)
+      if (int rc = check_matrix(y, rows, cols, ldy, "rmsnorm y")) return rc;
+    if (format)
+      if (int rc = check_mx(codes, scales, "rmsnorm result")) return rc;
+  }
+  OperatorDevice d;
+  if (int rc = operator_device(dev, &d)) return rc;
+  if (empty) return SB200_OK;
+  if (int rc = matrix_extent(dev, x, rows, cols, ldx, "rmsnorm x")) return rc;
+  if (int rc = matrix_extent(dev, weight, 1, cols, cols, "rmsnorm weight")) return rc;
+  if (int rc = matrix_extent(dev, residual, rows, cols, ldr, "rmsnorm residual")) return rc;
+  if (int rc = matrix_extent(dev, sum, rows, cols, lds, "rmsnorm sum")) return rc;
+  if (int rc = matrix_extent(dev, y, rows, cols, ldy, "rmsnorm y")) return rc;
   if (format)
-    if (int rc = check_mx(dev, format, rows, cols, codes, scales, "rmsnorm result")) return rc;
+    if (int rc = mx_extent(dev, format, rows, cols, codes, scales, "rmsnorm result")) return rc;
   RmsNorm p;
   memset(&p, 0, sizeof p);
   p.x = as_ptr<const float>(x);
@@ -433,33 +471,40 @@ int sb200_rmsnorm_workspace_bytes(int64_t rows, int64_t cols, uint64_t* bytes) {
 int sb200_rmsnorm_backward_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint64_t sum, int64_t lds, uint64_t weight, double eps,
                                uint64_t dy, int64_t lddy, uint64_t dsum, int64_t ldds, uint64_t dx, int64_t lddx, uint64_t dweight,
                                uint64_t workspace, uint64_t workspace_bytes) {
-  OperatorDevice d;
-  if (int rc = operator_device(dev, &d)) return rc;
   if (int rc = check_shape(rows, cols, "rmsnorm_backward")) return rc;
   if (!(eps >= 0.0)) return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm_backward: eps must not be negative");
-  if (cols == 0) return SB200_OK;
   if (!dx && !dweight) return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm_backward: no result asked for");
-  if (dweight)
-    if (int rc = check_matrix(dev, dweight, 1, cols, cols, "rmsnorm_backward dweight")) return rc;
+  const uint64_t need = static_cast<uint64_t>(dweight_parts(rows)) * cols * 4;
+  if (cols > 0 && dweight)
+    if (int rc = check_matrix(dweight, 1, cols, cols, "rmsnorm_backward dweight")) return rc;
+  if (cols > 0 && rows > 0) {
+    if (int rc = check_matrix(sum, rows, cols, lds, "rmsnorm_backward sum")) return rc;
+    if (int rc = check_matrix(weight, 1, cols, cols, "rmsnorm_backward weight")) return rc;
+    if (int rc = check_matrix(dy, rows, cols, lddy, "rmsnorm_backward dy")) return rc;
+    if (dsum)
+      if (int rc = check_matrix(dsum, rows, cols, ldds, "rmsnorm_backward dsum")) return rc;
+    if (dx)
+      if (int rc = check_matrix(dx, rows, cols, lddx, "rmsnorm_backward dx")) return rc;
+    if (dweight && (!workspace || workspace_bytes < need))
+      return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm_backward: dweight needs a workspace of %llu bytes", static_cast<unsigned long long>(need));
+    if (dweight && (workspace & 3)) return set_error(SB200_ERR_ALIGNMENT, "rmsnorm_backward: the workspace must be 4-byte aligned");
+  }
+  OperatorDevice d;
+  if (int rc = operator_device(dev, &d)) return rc;
+  if (cols == 0) return SB200_OK;
+  if (int rc = matrix_extent(dev, dweight, 1, cols, cols, "rmsnorm_backward dweight")) return rc;
   const cudaStream_t st = as_stream(stream);
   if (rows == 0) {  // an empty sum
     if (dweight) CU_TRY(cudaMemsetAsync(as_ptr<void>(dweight), 0, static_cast<size_t>(cols) * 4, st));
     return SB200_OK;
   }
-  if (int rc = check_matrix(dev, sum, rows, cols, lds, "rmsnorm_backward sum")) return rc;
-  if (int rc = check_matrix(dev, weight, 1, cols, cols, "rmsnorm_backward weight")) return rc;
-  if (int rc = check_matrix(dev, dy, rows, cols, lddy, "rmsnorm_backward dy")) return rc;
-  if (dsum)
-    if (int rc = check_matrix(dev, dsum, rows, cols, ldds, "rmsnorm_backward dsum")) return rc;
-  if (dx)
-    if (int rc = check_matrix(dev, dx, rows, cols, lddx, "rmsnorm_backward dx")) return rc;
-  if (dweight) {
-    const uint64_t need = static_cast<uint64_t>(dweight_parts(rows)) * cols * 4;
-    if (!workspace || workspace_bytes < need)
-      return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm_backward: dweight needs a workspace of %llu bytes", static_cast<unsigned long long>(need));
-    if (workspace & 3) return set_error(SB200_ERR_ALIGNMENT, "rmsnorm_backward: the workspace must be 4-byte aligned");
+  if (int rc = matrix_extent(dev, sum, rows, cols, lds, "rmsnorm_backward sum")) return rc;
+  if (int rc = matrix_extent(dev, weight, 1, cols, cols, "rmsnorm_backward weight")) return rc;
+  if (int rc = matrix_extent(dev, dy, rows, cols, lddy, "rmsnorm_backward dy")) return rc;
+  if (int rc = matrix_extent(dev, dsum, rows, cols, ldds, "rmsnorm_backward dsum")) return rc;
+  if (int rc = matrix_extent(dev, dx, rows, cols, lddx, "rmsnorm_backward dx")) return rc;
+  if (dweight)
     if (int rc = operator_extent(dev, workspace, need, "rmsnorm_backward workspace")) return rc;
-  }
   RmsNormBackward p;
   memset(&p, 0, sizeof p);
   p.h = as_ptr<const float>(sum);
