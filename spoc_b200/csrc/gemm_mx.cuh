@@ -334,7 +334,20 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
           cp += p.ldc;
         }
       };
-      if (!in_cluster && p.C && group < all) load_c(chunk_of(group));
+      if (!in_cluster && p.C) {
+        if (group < all) load_c(chunk_of(group));
+        // the lines of C that the chunks behind the first will read, into L2 under the k-loop: a lane a row
+        const float* ahead = p.C + static_cast<long long>(t0 + lane) * p.ldc + (f - lane);
+        if (f - lane < p.N) {
+          for (int n = group + 2; n < all; n += 2) {
+            const int c = chunk_of(n);
+            if (c + lane < rows) {
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(ahead + c * p.ldc));
+              if (f - lane + 31 < p.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(ahead + c * p.ldc + 31));
+            }
+          }
+        }
+      }
       const bool landed = mbar_wait_bounded(smem_u32(&tmem_full_bar[acc]), acc_phase, abort_flag);
       if (!__all_sync(0xffffffffu, landed)) {
         if (lane == 0) atomicCAS(p.status, 0, 0x2400 | (rank << 4) | acc);

@@ -81,13 +81,23 @@ __device__ __forceinline__ void mx_store_chunk(float4 v, uint32_t scale, uint8_t
   if ((lane & 7) == 0) scales[lane >> 3] = static_cast<uint8_t>(scale);
 }
 
-// Four values of a row from column `col` on; what is past `cols` counts for zero.  VEC: the row starts on 16 bytes and `cols` is a multiple of
-// four (the single elements beside the vectors cost the norm 30 registers a thread).
-template <bool VEC>
+// Four values of a row; what is past `cols` counts for zero.  A thread has columns col .. col + 3, col a multiple of four: as a vector (ACCESS_VECTOR: the
+// row starts on 16 bytes and `cols` is a multiple of four) or one by one (ACCESS_SINGLE); or, where it does not matter which thread has which
+// columns, a warp has its 128 columns with 32 of them side by side in the lanes (ACCESS_LANES), which takes a quarter of the lines a load.
+enum { ACCESS_SINGLE = 0, ACCESS_VECTOR = 1, ACCESS_LANES = 2 };
+template <int ACCESS>
 __device__ __forceinline__ float4 load4(const float* row, int col, int cols) {
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (VEC) {
+  if constexpr (ACCESS == ACCESS_VECTOR) {
     if (col < cols) v = *reinterpret_cast<const float4*>(row + col);
+    return v;
+  }
+  if constexpr (ACCESS == ACCESS_LANES) {
+    const int c = (col & ~127) + ((col & 127) >> 2);
+    if (c < cols) v.x = row[c];
+    if (c + 32 < cols) v.y = row[c + 32];
+    if (c + 64 < cols) v.z = row[c + 64];
+    if (c + 96 < cols) v.w = row[c + 96];
     return v;
   }
   if (col < cols) v.x = row[col];
@@ -96,10 +106,18 @@ __device__ __forceinline__ float4 load4(const float* row, int col, int cols) {
   if (col + 3 < cols) v.w = row[col + 3];
   return v;
 }
-template <bool VEC>
+template <int ACCESS>
 __device__ __forceinline__ void store4(float* row, int col, int cols, const float4& v) {
-  if (VEC) {
+  if constexpr (ACCESS == ACCESS_VECTOR) {
     if (col < cols) *reinterpret_cast<float4*>(row + col) = v;
+    return;
+  }
+  if constexpr (ACCESS == ACCESS_LANES) {
+    const int c = (col & ~127) + ((col & 127) >> 2);
+    if (c < cols) row[c] = v.x;
+    if (c + 32 < cols) row[c + 32] = v.y;
+    if (c + 64 < cols) row[c + 64] = v.z;
+    if (c + 96 < cols) row[c + 96] = v.w;
     return;
   }
   if (col < cols) row[col] = v.x;

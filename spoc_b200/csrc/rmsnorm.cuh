@@ -4,9 +4,9 @@
 //
 // A code of 8 or 4 bits is the rounding of the exact y of the stored h, with the sum of squares and the root in 64 bits: next to a rounding border
 // float32 falls on one side or the other depending on the order of the sum, one value in a million by a whole step, and so would all that is
-// computed from it.  64 bits throughout are not needed for that: y in float32 is at most seven units in the last place off (four from rsqrtf, two
-// products, the mean), and where a value of a warp's chunk lies within 16 of a border, or outside the range in which this holds, the warp does
-// the chunk over in 64 bits (rmsnorm_chunk_exact), one chunk of 250.
+// computed from it.  64 bits throughout are not needed for that: y in float32 is at most four units in the last place off (two products, and the
+// scale, which is two of 2^-24 off), and where a value of a warp's chunk lies within RMS_DOUBT of a border, or outside the range in which this
+// holds, the warp does the chunk over in 64 bits (rmsnorm_chunk_exact), one chunk of 700.
 //
 // A block a row, or a warp up to 1024 columns, the row in registers (VECS float4 a thread; thread t has columns 4 (v * threads + t)), so that x
 // and residual are read once.  Rows too long for that (32768 columns on) are read twice.  Bound by HBM: 8 bytes read, 5 written a value with
@@ -18,6 +18,8 @@
 #include "microscale.cuh"
 
 namespace sb200 {
+
+constexpr uint32_t RMS_DOUBT = 6;  // units in the last place
 
 struct RmsNorm {
   const float *x, *residual, *weight;  // residual may be null
@@ -61,20 +63,21 @@ __device__ __noinline__ void rmsnorm_chunk_exact(float4 h, float4 w, double mean
   mx_store_chunk<FP4>(y, mx_scale_of<FP4>(largest_of_block(y)), codes, scales, lane);
 }
 
-// Whether q, scaled for the type, lies so near the middle between two of its values that 16 units in the last place decide.  Below the type's
+// Whether q, scaled for the type, lies so near the middle between two of its values that RMS_DOUBT units in the last place decide.  Below the type's
 // smallest normal value (2^-6, 1) the values are as far apart as right above it: moved there, all middles are the same pattern of the bits
 // that the rounding drops.
 template <bool FP4>
 __device__ __forceinline__ bool near_middle(float q) {
   constexpr uint32_t DROPPED = FP4 ? 22 : 20;
   const float smallest = FP4 ? 1.0f : 0.015625f, a = fabsf(q), v = a < smallest ? a + smallest : a;
-  return ((__float_as_uint(v) + 16u - (1u << (DROPPED - 1))) & ((1u << DROPPED) - 1u)) <= 32u;
+  return ((__float_as_uint(v) + RMS_DOUBT - (1u << (DROPPED - 1))) & ((1u << DROPPED) - 1u)) <= 2 * RMS_DOUBT;
 }
 
 // What a row's results need.
 struct RmsRow {
   double mean;      // of the squares, plus eps
-  float scale;      // 1 / sqrt(mean), nearly
+  float unit;       // 1, or a power of two that brings values of a mean far from 1 near to it
+  float scale;      // 1 / (unit * sqrt(mean)), nearly
   float* y;         // each result's row, or null
   uint8_t *codes, *scales;
 };
@@ -82,19 +85,23 @@ template <int FORMAT>
 __device__ __forceinline__ RmsRow rmsnorm_row(const RmsNorm& p, long long row, double sum) {
   RmsRow r;
   r.mean = fma(sum, p.inv_cols, p.eps);
-  r.scale = rsqrtf(static_cast<float>(r.mean));
+  const int half = (static_cast<int>(__double2hiint(r.mean) >> 20 & 0x7ff) - 1023) / 2;
+  r.unit = abs(half) < 45 ? 1.0f : __uint_as_float(static_cast<uint32_t>(min(max(127 - half, 1), 254)) << 23);
+  // rsqrtf is two units in the last place off; a step of Newton's leaves the error of its own two roundings
+  const float m = static_cast<float>(r.mean * r.unit * r.unit), s = rsqrtf(m), e = fmaf(-m * s, s, 1.0f);
+  r.scale = s > 0.0f ? fmaf(0.5f * s, e, s) : s;  // of an infinite mean 0
   r.y = p.y ? p.y + row * p.ldy : nullptr;
   r.codes = p.codes + row * p.chunks * (FORMAT == 4 ? 64 : 128);
   r.scales = p.scales + mx_scale_offset(row, 0, p.chunks);
   return r;
 }
 // Four values of the normed row from column `col` on.  FORMAT: 0 float32 only, 4, 8.
-template <int FORMAT, bool VEC>
+template <int FORMAT, int ACCESS>
 __device__ __forceinline__ void rmsnorm_emit(const RmsNorm& p, const RmsRow& row, int col, const float4& h, int lane) {
-  const float s = row.scale;
-  const float4 w = load4<VEC>(p.weight, col, p.cols);
-  const float4 y = make_float4(h.x * s * w.x, h.y * s * w.y, h.z * s * w.z, h.w * s * w.w);
-  if (row.y) store4<VEC>(row.y, col, p.cols, y);
+  const float u = row.unit, s = row.scale;
+  const float4 w = load4<ACCESS>(p.weight, col, p.cols);
+  const float4 y = make_float4(h.x * u * s * w.x, h.y * u * s * w.y, h.z * u * s * w.z, h.w * u * s * w.w);
+  if (row.y) store4<ACCESS>(row.y, col, p.cols, y);
   if constexpr (FORMAT != 0) {
     constexpr bool FP4 = FORMAT == 4;
     const int chunk = col / MX_CHUNK;  // the same in a whole warp
@@ -108,29 +115,29 @@ __device__ __forceinline__ void rmsnorm_emit(const RmsNorm& p, const RmsRow& row
     bool again = near_middle<FP4>(y.x * f) || near_middle<FP4>(y.y * f) || near_middle<FP4>(y.z * f) || near_middle<FP4>(y.w * f);
     again = again || !(fmaxf(fmaxf(fabsf(w.x), fabsf(w.y)), fmaxf(fabsf(w.z), fabsf(w.w))) < 1.09951163e12f);
     again = again || (m == 0 ? (abs_bits(h.x) | abs_bits(h.y) | abs_bits(h.z) | abs_bits(h.w)) != 0
-                             : m - (67u << 23) >= 160u << 23 || ((m + 16u) & 0x7fffffu) <= 32u);  // next to a power of two the scale is in question
+                             : m - (67u << 23) >= 160u << 23 || ((m + RMS_DOUBT) & 0x7fffffu) <= 2 * RMS_DOUBT);  // next to a power of two the scale is in question
     if (__any_sync(0xffffffffu, again))
       rmsnorm_chunk_exact<FP4>(h, w, row.mean, codes, scales, lane);
     else
       mx_store_chunk<FP4>(y, block_scale, codes, scales, lane);
   }
 }
-__device__ __forceinline__ double squares(const float4& h) {
-  return fma(static_cast<double>(h.x), static_cast<double>(h.x), static_cast<double>(h.y) * h.y) +
-         fma(static_cast<double>(h.z), static_cast<double>(h.z), static_cast<double>(h.w) * h.w);
-}
-template <bool VEC>
+template <int ACCESS>
 __device__ __forceinline__ float4 rmsnorm_input(const RmsNorm& p, long long row, int col) {
-  float4 h = load4<VEC>(p.x + row * p.ldx, col, p.cols);
+  float4 h = load4<ACCESS>(p.x + row * p.ldx, col, p.cols);
   if (p.residual) {
-    const float4 r = load4<VEC>(p.residual + row * p.ldr, col, p.cols);
+    const float4 r = load4<ACCESS>(p.residual + row * p.ldr, col, p.cols);
     h = make_float4(__fadd_rn(h.x, r.x), __fadd_rn(h.y, r.y), __fadd_rn(h.z, r.z), __fadd_rn(h.w, r.w));
   }
   return h;
 }
+__device__ __forceinline__ double squares(const float4& h) {
+  return fma(static_cast<double>(h.x), static_cast<double>(h.x), static_cast<double>(h.y) * h.y) +
+         fma(static_cast<double>(h.z), static_cast<double>(h.z), static_cast<double>(h.w) * h.w);
+}
 // THREADS: of a row; 32: a block has four rows.  VECS = 0: rows of any length, read twice (h may be x or residual itself: then the second
 // reading takes h, which was stored).
-template <int FORMAT, int THREADS, int VECS, bool VEC, int BLOCKS>
+template <int FORMAT, int THREADS, int VECS, int ACCESS, int BLOCKS>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS, BLOCKS) rmsnorm_kernel(const RmsNorm p) {
   constexpr int ROWS = THREADS == 32 ? 4 : 1;
   __shared__ double shared[2][THREADS / 32];
@@ -148,29 +155,32 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS, BLOCKS) rmsnorm
     if constexpr (VECS > 0) {
       float4 h[VECS];
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) h[v] = rmsnorm_input<VEC>(p, row, first + v * 4 * THREADS);
+      for (int v = 0; v < VECS; ++v) h[v] = rmsnorm_input<ACCESS>(p, row, first + v * 4 * THREADS);
       double s = 0.0;
 #pragma unroll
       for (int v = 0; v < VECS; ++v) s += squares(h[v]);
       if (p.h) {
         float* to = p.h + row * p.ldh;
 #pragma unroll
-        for (int v = 0; v < VECS; ++v) store4<VEC>(to, first + v * 4 * THREADS, p.cols, h[v]);
+        for (int v = 0; v < VECS; ++v) store4<ACCESS>(to, first + v * 4 * THREADS, p.cols, h[v]);
       }
       const RmsRow r = rmsnorm_row<FORMAT>(p, row, block_sum<THREADS>(s, shared[turn]));
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) rmsnorm_emit<FORMAT, VEC>(p, r, first + v * 4 * THREADS, h[v], lane);
+      for (int v = 0; v < VECS; ++v) rmsnorm_emit<FORMAT, ACCESS>(p, r, first + v * 4 * THREADS, h[v], lane);
     } else {
+      const long long padded = static_cast<long long>(p.chunks) * MX_CHUNK;
       double s = 0.0;
-      for (long long col = first; col < p.cols; col += 4 * THREADS) {
-        const float4 h = rmsnorm_input<VEC>(p, row, static_cast<int>(col));
+      for (long long c = first; c < padded; c += 4 * THREADS) {
+        const int col = static_cast<int>(c);
+        const float4 h = rmsnorm_input<ACCESS>(p, row, col);
         s += squares(h);
-        if (p.h) store4<VEC>(p.h + row * p.ldh, static_cast<int>(col), p.cols, h);
+        if (p.h) store4<ACCESS>(p.h + row * p.ldh, col, p.cols, h);
       }
       const RmsRow r = rmsnorm_row<FORMAT>(p, row, block_sum<THREADS>(s, shared[turn]));
-      for (long long col = first; col < static_cast<long long>(p.chunks) * MX_CHUNK; col += 4 * THREADS) {
-        const float4 h = p.h ? load4<VEC>(p.h + row * p.ldh, static_cast<int>(col), p.cols) : rmsnorm_input<VEC>(p, row, static_cast<int>(col));
-        rmsnorm_emit<FORMAT, VEC>(p, r, static_cast<int>(col), h, lane);
+      for (long long c = first; c < padded; c += 4 * THREADS) {
+        const int col = static_cast<int>(c);
+        const float4 h = p.h ? load4<ACCESS>(p.h + row * p.ldh, col, p.cols) : rmsnorm_input<ACCESS>(p, row, col);
+        rmsnorm_emit<FORMAT, ACCESS>(p, r, col, h, lane);
       }
     }
   }
@@ -189,14 +199,15 @@ struct RmsNormBackward {
   int cols;
   double eps;
 };
-template <int THREADS, int VECS, bool VEC>
+template <int THREADS, int VECS, int ACCESS>
 __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNormBackward p) {
   __shared__ float2 shared[2][THREADS / 32];
   grid_launch_dependents();
   grid_dependency_wait();
   const int first = 4 * threadIdx.x;
   const float inv_cols = 1.0f / static_cast<float>(p.cols), eps = static_cast<float>(p.eps);
-  constexpr int HELD = VECS > 0 ? VECS : 1;
+  constexpr int HELD = VECS > 0 ? VECS : 1, PART = ACCESS == ACCESS_VECTOR ? ACCESS_SINGLE : ACCESS;  // the workspace starts on 4 bytes
+  const long long padded = (p.cols + 127ll) / 128 * 128;
   float4 part[HELD];
 #pragma unroll
   for (int v = 0; v < HELD; ++v) part[v] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -213,15 +224,15 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
     if constexpr (VECS > 0) {
 #pragma unroll
       for (int v = 0; v < VECS; ++v) {
-        h[v] = load4<VEC>(hr, first + v * 4 * THREADS, p.cols);
-        dy[v] = load4<VEC>(dyr, first + v * 4 * THREADS, p.cols);
+        h[v] = load4<ACCESS>(hr, first + v * 4 * THREADS, p.cols);
+        dy[v] = load4<ACCESS>(dyr, first + v * 4 * THREADS, p.cols);
       }
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) count(h[v], dy[v], load4<VEC>(p.weight, first + v * 4 * THREADS, p.cols));
+      for (int v = 0; v < VECS; ++v) count(h[v], dy[v], load4<ACCESS>(p.weight, first + v * 4 * THREADS, p.cols));
     } else {
-      for (long long c = first; c < p.cols; c += 4 * THREADS) {
+      for (long long c = first; c < padded; c += 4 * THREADS) {
         const int col = static_cast<int>(c);
-        count(load4<VEC>(hr, col, p.cols), load4<VEC>(dyr, col, p.cols), load4<VEC>(p.weight, col, p.cols));
+        count(load4<ACCESS>(hr, col, p.cols), load4<ACCESS>(dyr, col, p.cols), load4<ACCESS>(p.weight, col, p.cols));
       }
     }
 #pragma unroll
@@ -241,14 +252,14 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
     const float along = s.y * inv_cols * r * r;  // mean(g n) r: what h is multiplied by
     auto finish = [&](int col, const float4& a, const float4& d, float4& w_part) {
       if (p.dx) {
-        const float4 w = load4<VEC>(p.weight, col, p.cols);
+        const float4 w = load4<ACCESS>(p.weight, col, p.cols);
         float4 o = make_float4(r * fmaf(-a.x, along, d.x * w.x), r * fmaf(-a.y, along, d.y * w.y), r * fmaf(-a.z, along, d.z * w.z),
                                r * fmaf(-a.w, along, d.w * w.w));
         if (p.dsum) {
-          const float4 t = load4<VEC>(p.dsum + row * p.ldds, col, p.cols);
+          const float4 t = load4<ACCESS>(p.dsum + row * p.ldds, col, p.cols);
           o = make_float4(o.x + t.x, o.y + t.y, o.z + t.z, o.w + t.w);
         }
-        store4<VEC>(p.dx + row * p.lddx, col, p.cols, o);
+        store4<ACCESS>(p.dx + row * p.lddx, col, p.cols, o);
       }
       w_part.x = fmaf(d.x, a.x * r, w_part.x);
       w_part.y = fmaf(d.y, a.y * r, w_part.y);
@@ -259,22 +270,20 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
 #pragma unroll
       for (int v = 0; v < VECS; ++v) finish(first + v * 4 * THREADS, h[v], dy[v], part[v]);
     } else {
-      for (long long c = first; c < p.cols; c += 4 * THREADS) {
+      for (long long c = first; c < padded; c += 4 * THREADS) {
         const int col = static_cast<int>(c);
         float4 w_part = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p.dweight && row != blockIdx.x)
-          w_part = make_float4(mine[col], col + 1 < p.cols ? mine[col + 1] : 0.f, col + 2 < p.cols ? mine[col + 2] : 0.f,
-                               col + 3 < p.cols ? mine[col + 3] : 0.f);
-        const float4 a = load4<VEC>(hr, col, p.cols), d = load4<VEC>(dyr, col, p.cols);
+        if (p.dweight && row != blockIdx.x) w_part = load4<PART>(mine, col, p.cols);
+        const float4 a = load4<ACCESS>(hr, col, p.cols), d = load4<ACCESS>(dyr, col, p.cols);
         finish(col, a, d, w_part);
-        if (p.dweight) store4<false>(mine, col, p.cols, w_part);
+        if (p.dweight) store4<PART>(mine, col, p.cols, w_part);
       }
     }
   }
   if constexpr (VECS > 0) {
     if (p.dweight) {
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) store4<false>(mine, first + v * 4 * THREADS, p.cols, part[v]);
+      for (int v = 0; v < VECS; ++v) store4<PART>(mine, first + v * 4 * THREADS, p.cols, part[v]);
     }
   }
 }
@@ -324,7 +333,7 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
   float4 w[VECS], part[VECS];
 #pragma unroll
   for (int v = 0; v < VECS; ++v) {
-    w[v] = load4<true>(p.weight, first + v * 4 * TG, p.cols);
+    w[v] = load4<ACCESS_VECTOR>(p.weight, first + v * 4 * TG, p.cols);
     part[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   int stage = 0, turn = 0;
@@ -375,7 +384,7 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
       if (p.dx) {
         const float4 o = make_float4(r * fmaf(-a.x, along, d.x * w[v].x) + ds[v].x, r * fmaf(-a.y, along, d.y * w[v].y) + ds[v].y,
                                      r * fmaf(-a.z, along, d.z * w[v].z) + ds[v].z, r * fmaf(-a.w, along, d.w * w[v].w) + ds[v].w);
-        store4<true>(p.dx + row * p.lddx, first + v * 4 * TG, p.cols, o);
+        store4<ACCESS_VECTOR>(p.dx + row * p.lddx, first + v * 4 * TG, p.cols, o);
       }
       part[v].x = fmaf(d.x, a.x * r, part[v].x);
       part[v].y = fmaf(d.y, a.y * r, part[v].y);
@@ -395,7 +404,7 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
   float* const to = p.workspace + static_cast<long long>(blockIdx.x) * p.cols;
   if (G == 1) {
 #pragma unroll
-    for (int v = 0; v < VECS; ++v) store4<false>(to, first + v * 4 * TG, p.cols, part[v]);
+    for (int v = 0; v < VECS; ++v) store4<ACCESS_SINGLE>(to, first + v * 4 * TG, p.cols, part[v]);
     return;
   }
   __syncthreads();  // no copy is in flight: every group has waited for all that it asked for

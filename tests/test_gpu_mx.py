@@ -317,8 +317,11 @@ def test_norm_of_the_smallest_and_the_largest(keep, device, fmt, x_scale, w_scal
     rng = np.random.default_rng(2)
     x, w = (rng.normal(size=(4, 300)) * x_scale).astype(np.float32), (rng.normal(size=300) * w_scale).astype(np.float32)
     w[:40] *= np.float32(1e-6)
-    _, _, q = run_norm(keep, device, x, None, w, 0.0, fmt)
-    codes, scales = R.quantize(R.rmsnorm(x, None, w, 0.0)[1], fmt)
+    _, y, q = run_norm(keep, device, x, None, w, 0.0, fmt)
+    want = R.rmsnorm(x, None, w, 0.0)[1]
+    # as in test_norm, and a rounding to float32's smallest values, which a weight of a normal size keeps small
+    assert np.all(np.abs(y - want) <= 6 * 2.0 ** -23 * np.abs(want) + 2.0 ** -148 * np.maximum(1, np.abs(w)))
+    codes, scales = R.quantize(want, fmt)
     assert np.array_equal(q[1], scales) and np.array_equal(q[0], codes)
 
 
