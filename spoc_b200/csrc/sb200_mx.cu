@@ -206,7 +206,10 @@ template <bool FP4, int CTAS, int GROUPS, bool IN_CLUSTER = false>
 int launch_mx(const OperatorDevice& d, cudaStream_t st, const CUtensorMap (&maps)[6], const MxGemm& p) {
   auto kernel = gemm_mx_kernel<FP4, CTAS, GROUPS, IN_CLUSTER>;
   constexpr int kMost = 1024 + MXG_CTRL_BYTES + MXG_RING_BYTES;
-  const int smem = 1024 + MXG_CTRL_BYTES + std::max(p.stages * p.stage_bytes, IN_CLUSTER ? p.bt * 512 : 0);
+  // Blocks that wait for one another hold tensor memory while they do.  If two such blocks fitted an SM, the clusters of two launches on different
+  // streams could each have allocated on one SM and wait for the other on the next, for good: each takes more than half of the shared memory.
+  constexpr int kAlone = CTAS == 2 || IN_CLUSTER ? 114 * 1024 : 0;
+  const int smem = std::max(kAlone, 1024 + MXG_CTRL_BYTES + std::max(p.stages * p.stage_bytes, IN_CLUSTER ? p.bt * 512 : 0));
   static std::atomic<bool> ready[kMaxDevices];
   if (!ready[d.index].load()) {
     CU_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
