@@ -287,19 +287,23 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
     }
   }
 }
-// The same for rows that TMA can copy (16-byte aligned, a multiple of four values) and a block's registers hold: groups of TG threads go from row to
-// row, each with a ring of STAGES rows of h, dy and dsum in shared memory that bulk copies fill ahead of it, so that the copies of one row run
-// under the sums of another (8192 x 4096: 131 us with a row's loads in front of its sums, see the table of times in the launch function).
-template <int TG, int G, int VECS, int STAGES>
+// The same for rows that a block's registers hold: groups of TG threads go from row to row, each with a ring of STAGES rows of h, dy and dsum in
+// shared memory that bulk copies fill ahead of it, so that the copies of one row run under the sums of another (8192 x 4096 131 us with a
+// row's loads in front of its sums, 90 so).  ACCESS_LANES: rows that do not all start on 16 bytes.  Copies then begin and end at the multiples of 16
+// bytes around a row; the few bytes beside it are neither used nor beyond the 16 bytes of its first and last value.
+__device__ __forceinline__ uint32_t bulk_offset(const float* row) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) >> 2 & 3); }
+template <int TG, int G, int VECS, int STAGES, int ACCESS>
 struct BackwardRing {
   static constexpr int kThreads = TG * G, kCols = TG * VECS * 4;
-  static constexpr int kArrayBytes = kCols * 4, kStageBytes = 3 * kArrayBytes;
+  static constexpr int kArrayBytes = kCols * 4 + (ACCESS == ACCESS_LANES ? 32 : 0), kStageBytes = 3 * kArrayBytes;
   static constexpr int kBytes = G * STAGES * kStageBytes + 128;  // the copies start on 128 bytes
-  static_assert(G * kArrayBytes <= G * STAGES * kStageBytes, "the groups' parts of dweight fit the ring");
+  static_assert(G * kCols * 4 <= G * STAGES * kStageBytes, "the groups' parts of dweight fit the ring");
+  static_assert(kArrayBytes % 16 == 0, "copies start on 16 bytes");
 };
-template <int TG, int G, int VECS, int STAGES, int BLOCKS>
+template <int TG, int G, int VECS, int STAGES, int BLOCKS, int ACCESS>
 __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(const RmsNormBackward p) {
-  using Ring = BackwardRing<TG, G, VECS, STAGES>;
+  using Ring = BackwardRing<TG, G, VECS, STAGES, ACCESS>;
+  constexpr int PART = ACCESS == ACCESS_VECTOR ? ACCESS_SINGLE : ACCESS;  // the workspace starts on 4 bytes
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[G * STAGES];
   __shared__ float2 sums[2][G * TG / 32];
@@ -320,10 +324,15 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
   const uint32_t bytes = static_cast<uint32_t>(p.cols) * 4;
   auto fetch = [&](int stage, long long row) {  // one thread
     const uint32_t bar = smem_u32(&full[group * STAGES + stage]), to = smem_u32(mine) + stage * Ring::kStageBytes;
-    mbar_arrive_expect_tx(bar, p.dsum ? 3 * bytes : 2 * bytes);
-    bulk_load(to, p.h + row * p.ldh, bytes, bar);
-    bulk_load(to + Ring::kArrayBytes, p.dy + row * p.lddy, bytes, bar);
-    if (p.dsum) bulk_load(to + 2 * Ring::kArrayBytes, p.dsum + row * p.ldds, bytes, bar);
+    auto size = [&](const float* from) { return ((ACCESS == ACCESS_VECTOR ? 0u : bulk_offset(from)) * 4 + bytes + 15) & ~15u; };
+    auto copy = [&](int array, const float* from) {
+      bulk_load(to + array * Ring::kArrayBytes, ACCESS == ACCESS_VECTOR ? from : from - bulk_offset(from), size(from), bar);
+    };
+    const float *h = p.h + row * p.ldh, *dy = p.dy + row * p.lddy, *ds = p.dsum + row * p.ldds;
+    mbar_arrive_expect_tx(bar, size(h) + size(dy) + (p.dsum ? size(ds) : 0));
+    copy(0, h);
+    copy(1, dy);
+    if (p.dsum) copy(2, ds);
   };
   if (thread == 0) {
 #pragma unroll 1
@@ -333,7 +342,7 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
   float4 w[VECS], part[VECS];
 #pragma unroll
   for (int v = 0; v < VECS; ++v) {
-    w[v] = load4<ACCESS_VECTOR>(p.weight, first + v * 4 * TG, p.cols);
+    w[v] = load4<ACCESS>(p.weight, first + v * 4 * TG, p.cols);
     part[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   int stage = 0, turn = 0;
@@ -347,11 +356,18 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
       const int col = first + v * 4 * TG;
+      const float* const at = reinterpret_cast<const float*>(from);
       h[v] = dy[v] = ds[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (col < p.cols) {
-        h[v] = *reinterpret_cast<const float4*>(from + col * 4);
-        dy[v] = *reinterpret_cast<const float4*>(from + Ring::kArrayBytes + col * 4);
-        if (p.dsum) ds[v] = *reinterpret_cast<const float4*>(from + 2 * Ring::kArrayBytes + col * 4);
+      if constexpr (ACCESS == ACCESS_VECTOR) {
+        if (col < p.cols) {
+          h[v] = *reinterpret_cast<const float4*>(at + col);
+          dy[v] = *reinterpret_cast<const float4*>(at + Ring::kArrayBytes / 4 + col);
+          if (p.dsum) ds[v] = *reinterpret_cast<const float4*>(at + 2 * (Ring::kArrayBytes / 4) + col);
+        }
+      } else {
+        h[v] = load4<ACCESS>(at + bulk_offset(p.h + row * p.ldh), col, p.cols);
+        dy[v] = load4<ACCESS>(at + Ring::kArrayBytes / 4 + bulk_offset(p.dy + row * p.lddy), col, p.cols);
+        if (p.dsum) ds[v] = load4<ACCESS>(at + 2 * (Ring::kArrayBytes / 4) + bulk_offset(p.dsum + row * p.ldds), col, p.cols);
       }
       const float4 &a = h[v], &d = dy[v];
       s.x += fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w);
@@ -384,7 +400,7 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
       if (p.dx) {
         const float4 o = make_float4(r * fmaf(-a.x, along, d.x * w[v].x) + ds[v].x, r * fmaf(-a.y, along, d.y * w[v].y) + ds[v].y,
                                      r * fmaf(-a.z, along, d.z * w[v].z) + ds[v].z, r * fmaf(-a.w, along, d.w * w[v].w) + ds[v].w);
-        store4<ACCESS_VECTOR>(p.dx + row * p.lddx, first + v * 4 * TG, p.cols, o);
+        store4<ACCESS>(p.dx + row * p.lddx, first + v * 4 * TG, p.cols, o);
       }
       part[v].x = fmaf(d.x, a.x * r, part[v].x);
       part[v].y = fmaf(d.y, a.y * r, part[v].y);
@@ -404,13 +420,13 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
   float* const to = p.workspace + static_cast<long long>(blockIdx.x) * p.cols;
   if (G == 1) {
 #pragma unroll
-    for (int v = 0; v < VECS; ++v) store4<ACCESS_SINGLE>(to, first + v * 4 * TG, p.cols, part[v]);
+    for (int v = 0; v < VECS; ++v) store4<PART>(to, first + v * 4 * TG, p.cols, part[v]);
     return;
   }
   __syncthreads();  // no copy is in flight: every group has waited for all that it asked for
   float* const shared_part = reinterpret_cast<float*>(ring);
 #pragma unroll
-  for (int v = 0; v < VECS; ++v) *reinterpret_cast<float4*>(shared_part + group * Ring::kCols + first + v * 4 * TG) = part[v];
+  for (int v = 0; v < VECS; ++v) store4<ACCESS>(shared_part + group * Ring::kCols, first + v * 4 * TG, Ring::kCols, part[v]);
   __syncthreads();
   for (int c = threadIdx.x; c < p.cols; c += TG * G) {
     float s = 0.0f;

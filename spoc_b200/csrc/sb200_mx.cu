@@ -113,10 +113,10 @@ int launch_rmsnorm(int sm_count, cudaStream_t st, const RmsNorm& p) {
 
 int64_t dweight_parts(int64_t rows) { return std::min<int64_t>(rows, SB200_RMSNORM_MAX_PARTS); }
 
-template <int TG, int G, int VECS, int STAGES, int BLOCKS>
+template <int TG, int G, int VECS, int STAGES, int BLOCKS, int ACCESS>
 int launch_backward_ring(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, unsigned* grid) {
-  using Ring = BackwardRing<TG, G, VECS, STAGES>;
-  auto kernel = rmsnorm_backward_ring_kernel<TG, G, VECS, STAGES, BLOCKS>;
+  using Ring = BackwardRing<TG, G, VECS, STAGES, ACCESS>;
+  auto kernel = rmsnorm_backward_ring_kernel<TG, G, VECS, STAGES, BLOCKS, ACCESS>;
   static std::atomic<bool> ready[kMaxDevices];
   if (!ready[d.index].load()) {
     CU_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring::kBytes));
@@ -127,26 +127,22 @@ int launch_backward_ring(const OperatorDevice& d, cudaStream_t st, const RmsNorm
   CU_TRY(launch_pdl(kernel, dim3(*grid), dim3(TG * G), Ring::kBytes, st, 1, p));
   return operator_launched("rmsnorm_backward_ring_kernel");
 }
+template <int ACCESS>
 int launch_backward_rings(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, unsigned* grid) {
   const int cols = p.cols;
-  if (cols <= 128) return launch_backward_ring<32, 8, 1, 4, 3>(d, st, p, grid);
-  if (cols <= 512) return launch_backward_ring<128, 2, 1, 5, 3>(d, st, p, grid);
-  if (cols <= 1024) return launch_backward_ring<256, 1, 1, 5, 3>(d, st, p, grid);
-  if (cols <= 2048) return launch_backward_ring<256, 1, 2, 3, 3>(d, st, p, grid);
-  if (cols <= 4096) return launch_backward_ring<512, 1, 2, 2, 2>(d, st, p, grid);
-  return launch_backward_ring<1024, 1, 2, 2, 1>(d, st, p, grid);
+  if (cols <= 128) return launch_backward_ring<32, 8, 1, 4, 3, ACCESS>(d, st, p, grid);
+  if (cols <= 512) return launch_backward_ring<128, 2, 1, 5, 3, ACCESS>(d, st, p, grid);
+  if (cols <= 1024) return launch_backward_ring<256, 1, 1, 5, 3, ACCESS>(d, st, p, grid);
+  if (cols <= 2048) return launch_backward_ring<256, 1, 2, 3, 3, ACCESS>(d, st, p, grid);
+  if (cols <= 4096) return launch_backward_ring<512, 1, 2, 2, 2, ACCESS>(d, st, p, grid);
+  return launch_backward_ring<1024, 1, 2, 2, 1, ACCESS>(d, st, p, grid);
 }
 template <bool VEC>
 int launch_backward_rows(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, unsigned* grid) {
   *grid = static_cast<unsigned>(std::min<int64_t>(dweight_parts(p.rows), static_cast<int64_t>(d.sm_count) * 2));
 #define SB200_NORM(THREADS, VECS) CU_TRY(launch_pdl(rmsnorm_backward_kernel<THREADS, VECS, VEC ? ACCESS_VECTOR : ACCESS_LANES>, dim3(*grid), dim3(THREADS), 0, st, 1, p))
   const int64_t cols = p.cols;
-  if (cols <= 512) SB200_NORM(128, 1);
-  else if (cols <= 1024) SB200_NORM(256, 1);
-  else if (cols <= 2048) SB200_NORM(256, 2);
-  else if (cols <= 4096) SB200_NORM(256, 4);
-  else if (cols <= 8192) SB200_NORM(512, 4);
-  else if (cols <= 16384) SB200_NORM(512, 8);
+  if (cols <= 16384) SB200_NORM(512, 8);
   else SB200_NORM(1024, 0);
 #undef SB200_NORM
   return operator_launched("rmsnorm_backward_kernel");
@@ -154,7 +150,7 @@ int launch_backward_rows(const OperatorDevice& d, cudaStream_t st, const RmsNorm
 int launch_rmsnorm_backward(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, bool vec) {
   unsigned grid = 0;
   int rc;
-  if (vec && p.cols <= 8192) rc = launch_backward_rings(d, st, p, &grid);
+  if (p.cols <= 8192) rc = vec ? launch_backward_rings<ACCESS_VECTOR>(d, st, p, &grid) : launch_backward_rings<ACCESS_LANES>(d, st, p, &grid);
   else rc = vec ? launch_backward_rows<true>(d, st, p, &grid) : launch_backward_rows<false>(d, st, p, &grid);
   if (rc || !p.dweight) return rc;
   CU_TRY(launch_pdl(rmsnorm_dweight_kernel, dim3(grid_for(p.cols, 32, 1 << 20)), dim3(256), 0, st, 1, static_cast<const float*>(p.workspace),
