@@ -602,3 +602,82 @@ def test_rows_and_columns_that_are_not_there_stay_as_they_are(keep, device):
 def test_errors_carry_the_message(keep, device):
     with pytest.raises(BackendError, match="leading dimension"):
         gemm_mx(device, keep.mx(FP8, 4, 32), keep.mx(FP8, 9, 32), keep.out(36), ldd=8)
+
+
+# ------------------------------------------------------------------ far and wide
+def test_offsets_past_32_bits(keep, backend, device):
+    """Five rows 2^30 + 4 floats apart, the last of which lie beyond 2^32 elements: read, summed, written."""
+    rows, cols, ld = 5, 132, (1 << 30) + 4
+    lib = L.load()
+    rng = np.random.default_rng(0)
+    x, w = rng.normal(size=(rows, cols)).astype(np.float32), rng.normal(size=cols).astype(np.float32)
+    far = backend.Memory.alloc(device, (rows - 1) * ld + cols, np.float32)
+
+    def put(a):
+        for i in range(rows):
+            row = np.ascontiguousarray(a[i])
+            _check(lib.sb200_memcpy_htod(device.id, far.ptr + 4 * i * ld, row.ctypes.data_as(C.c_void_p), 4 * cols))
+
+    def get():
+        out = np.empty((rows, cols), np.float32)
+        for i in range(rows):
+            _check(lib.sb200_memcpy_dtoh(device.id, out[i].ctypes.data_as(C.c_void_p), far.ptr + 4 * i * ld, 4 * cols))
+        return out
+
+    try:
+        q, wd, dw, ws = keep.mx(FP8, rows, cols), keep.f32(w), keep.out(cols), keep.bytes(rows * cols * 4)
+        codes, scales = R.quantize(x, FP8)
+        put(x)
+        _check(lib.sb200_mx_quantize(device.id, 0, FP8, rows, cols, far.ptr, ld, 0, q.codes.ptr, q.scales.ptr))
+        assert np.array_equal(q.download()[0], codes) and np.array_equal(q.download()[1], scales)
+        put(np.zeros_like(x))
+        _check(lib.sb200_mx_dequantize(device.id, 0, FP8, rows, cols, q.codes.ptr, q.scales.ptr, far.ptr, ld))
+        assert np.array_equal(get(), R.values(codes, scales, FP8, cols).astype(np.float32))
+        turned = keep.mx(FP4, cols, rows)
+        put(x)
+        _check(lib.sb200_mx_quantize(device.id, 0, FP4, cols, rows, far.ptr, ld, 1, turned.codes.ptr, turned.scales.ptr))
+        assert np.array_equal(turned.download()[0], R.quantize(x.T, FP4)[0])
+        _check(lib.sb200_rmsnorm_f32(device.id, 0, rows, cols, far.ptr, ld, far.ptr, ld, wd.ptr, 1e-5, far.ptr, ld, 0, 0, FP8, q.codes.ptr, q.scales.ptr))
+        h, y = R.rmsnorm(x, x, w, 1e-5)
+        assert np.array_equal(get(), h) and np.array_equal(q.download()[0], R.quantize(y, FP8)[0])
+        _check(lib.sb200_rmsnorm_backward_f32(device.id, 0, rows, cols, far.ptr, ld, wd.ptr, 1e-5, far.ptr, ld, far.ptr, ld, far.ptr, ld, dw.ptr, ws.ptr,
+                                              rows * cols * 4))
+        backend.Device.synchronize(device)
+        check_backward((get(), dw.download()), h, w, h, h, 1e-5)
+        a, b = random_mx(rng, FP8, rows, 200), random_mx(rng, FP4, cols, 200)
+        A, B = keep.mx(FP8, rows, 200, a), keep.mx(FP4, cols, 200, b)
+        put(x)
+        _check(lib.sb200_gemm_mx(device.id, 0, FP8, FP4, rows, cols, 200, A.codes.ptr, A.scales.ptr, B.codes.ptr, B.scales.ptr, far.ptr, ld, 1.0, far.ptr, ld,
+                                 1.0, 0, 0))
+        backend.Device.synchronize(device)
+        va, vb = R.values(*a, FP8, 200), R.values(*b, FP4, 200)
+        assert np.all(np.abs(get() - (va @ vb.T + x)) <= (200 / 32 + 16) * 2.0 ** -23 * (np.abs(va) @ np.abs(vb).T + np.abs(x)))
+    finally:
+        backend.Memory.free(far)
+
+
+@pytest.mark.parametrize("m,n,k", [(70001, 5, 40), (3, 150001, 64), (1, 1, 70000), (130, 2, 40000), (2, 131, 33000)])
+def test_product_of_the_longest(keep, device, m, n, k):
+    check_product(keep, device, FP8, FP4, m, n, k, epilogue=True)
+
+
+@pytest.mark.parametrize("rows,cols", [(100003, 3), (1, 300001), (2, 262144), (65537, 36)])
+def test_norm_of_the_longest(keep, device, rows, cols):
+    rng = np.random.default_rng(cols)
+    x, r, w = norm_inputs(rng, rows, cols)
+    s, y, q = run_norm(keep, device, x, r, w, 1e-5, FP8)
+    h, want = R.rmsnorm(x, r, w, 1e-5)
+    codes, scales = R.quantize(want, FP8)
+    assert np.array_equal(s, h) and np.array_equal(q[0], codes) and np.array_equal(q[1], scales)
+    dy = rng.normal(size=(rows, cols)).astype(np.float32)
+    check_backward(run_backward(keep, device, h, w, dy, x, 1e-5), h, w, dy, x, 1e-5)
+
+
+@pytest.mark.parametrize("rows,k", [(100003, 1), (1, 300001), (3, 131072)])
+@pytest.mark.parametrize("transposed", [0, 1])
+def test_quantize_the_longest(keep, device, rows, k, transposed):
+    v = np.random.default_rng(k).normal(size=(rows, k)).astype(np.float32)
+    x, q = keep.f32(v.T if transposed else v), keep.mx(FP4, rows, k)
+    _check(L.load().sb200_mx_quantize(device.id, 0, FP4, rows, k, x.ptr, rows if transposed else k, transposed, q.codes.ptr, q.scales.ptr))
+    codes, scales = R.quantize(v, FP4)
+    assert np.array_equal(q.download()[0], codes) and np.array_equal(q.download()[1], scales)
