@@ -70,15 +70,19 @@ __device__ __forceinline__ uint32_t largest_of_block(const float4& v) {
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
   return max(m, __shfl_xor_sync(0xffffffffu, m, 4));
 }
-// codes: of the chunk; scales: its four.
+// codes: of the chunk; scales: its four; c: the lane's four codes, scale: of their block.
 template <bool FP4>
-__device__ __forceinline__ void mx_store_chunk(float4 v, uint32_t scale, uint8_t* codes, uint8_t* scales, int lane) {
-  const uint32_t c = mx_codes4<FP4>(v, mx_factor(scale));
+__device__ __forceinline__ void mx_store_codes(uint32_t c, uint32_t scale, uint8_t* codes, uint8_t* scales, int lane) {
   if constexpr (FP4)
     reinterpret_cast<uint16_t*>(codes)[lane] = static_cast<uint16_t>(c);
   else
     reinterpret_cast<uint32_t*>(codes)[lane] = c;
   if ((lane & 7) == 0) scales[lane >> 3] = static_cast<uint8_t>(scale);
+}
+
+template <bool FP4>
+__device__ __forceinline__ void mx_store_chunk(const float4& v, uint32_t scale, uint8_t* codes, uint8_t* scales, int lane) {
+  mx_store_codes<FP4>(mx_codes4<FP4>(v, mx_factor(scale)), scale, codes, scales, lane);
 }
 
 // Four values of a row; what is past `cols` counts for zero.  A thread has columns col .. col + 3, col a multiple of four: as a vector (ACCESS_VECTOR: the

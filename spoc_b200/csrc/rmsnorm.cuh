@@ -4,9 +4,9 @@
 //
 // A code of 8 or 4 bits is the rounding of the exact y of the stored h, with the sum of squares and the root in 64 bits: next to a rounding border
 // float32 falls on one side or the other depending on the order of the sum, one value in a million by a whole step, and so would all that is
-// computed from it.  64 bits throughout are not needed for that: y in float32 is at most four units in the last place off (two products, and the
-// scale, which is two of 2^-24 off), and where a value of a warp's chunk lies within RMS_DOUBT of a border, or outside the range in which this
-// holds, the warp does the chunk over in 64 bits (rmsnorm_chunk_exact), one chunk of 700.
+// computed from it.  64 bits throughout are not needed for that: y in float32 is at most 2^-22 of it off (two products, and the scale, which is two of
+// 2^-24 off).  Where a value of a warp's chunk has another code, or a block another scale, for 1 - RMS_DOUBT and 1 + RMS_DOUBT times it, or lies
+// outside the range in which this holds, the warp does the chunk over in 64 bits (rmsnorm_chunk_exact), one chunk of 600.
 //
 // A block a row, or a warp up to 1024 columns, the row in registers (VECS float4 a thread; thread t has columns 4 (v * threads + t)), so that x
 // and residual are read once.  Rows too long for that (32768 columns on) are read twice.  Bound by HBM: 8 bytes read, 5 written a value with
@@ -19,7 +19,7 @@
 
 namespace sb200 {
 
-constexpr uint32_t RMS_DOUBT = 6;  // units in the last place
+constexpr float RMS_DOUBT = 4.76837158203125e-7f;  // 2^-21
 
 struct RmsNorm {
   const float *x, *residual, *weight;  // residual may be null
@@ -39,9 +39,9 @@ __device__ __forceinline__ T block_sum(T v, T* shared) {
   if (THREADS == 32) return v;
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
-  T s = 0;
+  T s = shared[threadIdx.x & (THREADS / 32 - 1)];
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) s += shared[w];
+  for (int o = THREADS / 64; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
 
@@ -61,16 +61,6 @@ __device__ __noinline__ void rmsnorm_chunk_exact(float4 h, float4 w, double mean
   const float4 y = make_float4(round_to_odd(h.x * scale * w.x), round_to_odd(h.y * scale * w.y), round_to_odd(h.z * scale * w.z),
                                round_to_odd(h.w * scale * w.w));
   mx_store_chunk<FP4>(y, mx_scale_of<FP4>(largest_of_block(y)), codes, scales, lane);
-}
-
-// Whether q, scaled for the type, lies so near the middle between two of its values that RMS_DOUBT units in the last place decide.  Below the type's
-// smallest normal value (2^-6, 1) the values are as far apart as right above it: moved there, all middles are the same pattern of the bits
-// that the rounding drops.
-template <bool FP4>
-__device__ __forceinline__ bool near_middle(float q) {
-  constexpr uint32_t DROPPED = FP4 ? 22 : 20;
-  const float smallest = FP4 ? 1.0f : 0.015625f, a = fabsf(q), v = a < smallest ? a + smallest : a;
-  return ((__float_as_uint(v) + RMS_DOUBT - (1u << (DROPPED - 1))) & ((1u << DROPPED) - 1u)) <= 2 * RMS_DOUBT;
 }
 
 // What a row's results need.
@@ -98,9 +88,11 @@ __device__ __forceinline__ RmsRow rmsnorm_row(const RmsNorm& p, long long row, d
 // Four values of the normed row from column `col` on.  FORMAT: 0 float32 only, 4, 8.
 template <int FORMAT, int ACCESS>
 __device__ __forceinline__ void rmsnorm_emit(const RmsNorm& p, const RmsRow& row, int col, const float4& h, int lane) {
-  const float u = row.unit, s = row.scale;
+  const float s = row.scale;
   const float4 w = load4<ACCESS>(p.weight, col, p.cols);
-  const float4 y = make_float4(h.x * u * s * w.x, h.y * u * s * w.y, h.z * u * s * w.z, h.w * u * s * w.w);
+  float4 y = h;
+  if (row.unit != 1.0f) y = make_float4(h.x * row.unit, h.y * row.unit, h.z * row.unit, h.w * row.unit);
+  y = make_float4(y.x * s * w.x, y.y * s * w.y, y.z * s * w.z, y.w * s * w.w);
   if (row.y) store4<ACCESS>(row.y, col, p.cols, y);
   if constexpr (FORMAT != 0) {
     constexpr bool FP4 = FORMAT == 4;
@@ -109,17 +101,18 @@ __device__ __forceinline__ void rmsnorm_emit(const RmsNorm& p, const RmsRow& row
     uint8_t* codes = row.codes + static_cast<long long>(chunk) * MxFormat<FP4>::kChunkBytes;
     uint8_t* scales = row.scales + static_cast<long long>(chunk) * MX_TILE_BYTES;
     const uint32_t m = largest_of_block(y), block_scale = mx_scale_of<FP4>(m);
-    const float f = mx_factor(block_scale);
+    const float f = mx_factor(block_scale), top = __uint_as_float(m);
+    const uint32_t low = mx_codes4<FP4>(y, f * (1.0f - RMS_DOUBT)), high = mx_codes4<FP4>(y, f * (1.0f + RMS_DOUBT));
     // The estimate holds for weights below 2^40 and a largest value between 2^-60 and 2^100: products that fall below float32's range then lose
     // nothing that a code shows.  A block of zeros holds too, where h is zero.
-    bool again = near_middle<FP4>(y.x * f) || near_middle<FP4>(y.y * f) || near_middle<FP4>(y.z * f) || near_middle<FP4>(y.w * f);
-    again = again || !(fmaxf(fmaxf(fabsf(w.x), fabsf(w.y)), fmaxf(fabsf(w.z), fabsf(w.w))) < 1.09951163e12f);
+    bool again = low != high || !(fmaxf(fmaxf(fabsf(w.x), fabsf(w.y)), fmaxf(fabsf(w.z), fabsf(w.w))) < 1.09951163e12f);
     again = again || (m == 0 ? (abs_bits(h.x) | abs_bits(h.y) | abs_bits(h.z) | abs_bits(h.w)) != 0
-                             : m - (67u << 23) >= 160u << 23 || ((m + RMS_DOUBT) & 0x7fffffu) <= 2 * RMS_DOUBT);  // next to a power of two the scale is in question
+                             : m - (67u << 23) >= 160u << 23 ||
+                                   ((__float_as_uint(top * (1.0f - RMS_DOUBT)) ^ __float_as_uint(top * (1.0f + RMS_DOUBT))) >> 23) != 0);
     if (__any_sync(0xffffffffu, again))
       rmsnorm_chunk_exact<FP4>(h, w, row.mean, codes, scales, lane);
     else
-      mx_store_chunk<FP4>(y, block_scale, codes, scales, lane);
+      mx_store_codes<FP4>(low, block_scale, codes, scales, lane);
   }
 }
 template <int ACCESS>
