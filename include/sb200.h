@@ -433,8 +433,8 @@ SB200_API int sb200_mx_quantize(int dev, uint64_t stream, int format, int64_t ro
 SB200_API int sb200_mx_dequantize(int dev, uint64_t stream, int format, int64_t rows, int64_t K, uint64_t codes, uint64_t scales,
                                   uint64_t dst, int64_t ld);
 /* D[M x N] = act(alpha * A[M x K] . B[N x K]^T + beta * C[M x N] + bias[N]) of microscaled A and B in either format each, the sums float32;
- * D, C and bias as in sb200_gemm_f32 (C and bias may be 0, D may be C).  Gradients of y = x . W^T: dx = dy . W takes dy and W quantised along
- * N, dW = dy^T . x takes both quantised along M (`transposed`). */
+ * D, C and bias as in sb200_gemm_f32 (C and bias may be 0, D may be C at the same leading dimension).  Gradients of y = x . W^T:
+ * dx = dy . W takes dy and W quantised along N, dW = dy^T . x takes both quantised along M (`transposed`). */
 SB200_API int sb200_gemm_mx(int dev, uint64_t stream, int format_a, int format_b, int64_t M, int64_t N, int64_t K,
                             uint64_t a_codes, uint64_t a_scales, uint64_t b_codes, uint64_t b_scales,
                             uint64_t D, int64_t ldd, float alpha, uint64_t C, int64_t ldc, float beta, uint64_t bias, int act);
@@ -442,7 +442,8 @@ SB200_API int sb200_gemm_mx(int dev, uint64_t stream, int format_a, int format_b
 /* ---- root-mean-square norm ----------------------------------------------------------------------------
  * h = x + residual (rounded to float32; residual may be 0), y = h * weight / sqrt(mean(h^2) + eps), by rows of `cols`.  Results, each
  * optional: `sum` takes h, y the float32 result, codes and scales (format SB200_MX_FP8 or SB200_MX_FP4; 0: none) the microscaled one, whose
- * codes are roundings of y in 64 bits.  sum may be x or residual, and y may be x or residual, at the same leading dimension. */
+ * codes are roundings of y in 64 bits.  sum may be x or residual, and y may be x or residual, at the same leading dimension (with another it
+ * is SB200_ERR_INVALID_VALUE); sum and y are two matrices. */
 SB200_API int sb200_rmsnorm_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint64_t x, int64_t ldx, uint64_t residual, int64_t ldr,
                                 uint64_t weight, double eps, uint64_t sum, int64_t lds, uint64_t y, int64_t ldy,
                                 int format, uint64_t codes, uint64_t scales);
@@ -450,7 +451,9 @@ SB200_API int sb200_rmsnorm_f32(int dev, uint64_t stream, int64_t rows, int64_t 
  *   dx = dsum + r * (g - n * mean(g * n))  (the gradient of x and of residual),  dweight = sum over the rows of dy * n,
  * dsum the gradient that reaches `sum` from elsewhere (may be 0).  dx or dweight may be 0; dx may be dy, dsum or sum at the same leading
  * dimension.  dweight needs a workspace of sb200_rmsnorm_workspace_bytes: min(rows, 512) * cols * 4; calls that may run at the same
- * time need one each.  Results do not depend on timing. */
+ * time need one each.  Results do not depend on timing.  Sums are float32, those of the squares among them: values of `sum` beyond 1e18, and
+ * rows that lie below 1e-18 with an eps that small, are out of their range (the norm itself takes them).  Of no rows dweight is zero: a
+ * memset, where the other calls are kernel launches alone. */
 #define SB200_RMSNORM_MAX_PARTS 512
 SB200_API int sb200_rmsnorm_workspace_bytes(int64_t rows, int64_t cols, uint64_t *bytes);
 SB200_API int sb200_rmsnorm_backward_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint64_t sum, int64_t lds, uint64_t weight,

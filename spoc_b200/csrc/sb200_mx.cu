@@ -66,6 +66,11 @@ int check_matrix(uint64_t p, int64_t rows, int64_t cols, int64_t ld, const char*
   if (ld > INT64_MAX / 8 / (rows > 0 ? rows : 1)) return set_error(SB200_ERR_TOO_LARGE, "%s: extent beyond 64 bits", what);
   return SB200_OK;
 }
+// A result may be an operand itself, row on row: with other row lengths a row would be written before another block has read it.
+int check_in_place(uint64_t result, int64_t ldr, uint64_t operand, int64_t ldo, int64_t rows, const char* what) {
+  if (!result || result != operand || ldr == ldo || rows < 2) return SB200_OK;
+  return set_error(SB200_ERR_INVALID_VALUE, "%s: in place with another leading dimension (%lld, operand %lld)", what, (long long)ldr, (long long)ldo);
+}
 // What lies in a buffer of the library's ends there.
 int mx_extent(int dev, int format, int64_t rows, int64_t K, uint64_t codes, uint64_t scales, const char* what) {
   if (int rc = operator_extent(dev, codes, code_bytes(format, rows, K), what)) return rc;
@@ -377,6 +382,7 @@ int sb200_gemm_mx(int dev, uint64_t stream, int format_a, int format_b, int64_t 
     if (int rc = check_matrix(D, M, N, ldd, "gemm_mx result D")) return rc;
     if (C)
       if (int rc = check_matrix(C, M, N, ldc, "gemm_mx operand C")) return rc;
+    if (int rc = check_in_place(D, ldd, C, ldc, M, "gemm_mx")) return rc;
     if (bias)
       if (int rc = check_matrix(bias, 1, N, N, "gemm_mx bias")) return rc;
   }
@@ -428,6 +434,11 @@ int sb200_rmsnorm_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint
       if (int rc = check_matrix(y, rows, cols, ldy, "rmsnorm y")) return rc;
     if (format)
       if (int rc = check_mx(codes, scales, "rmsnorm result")) return rc;
+    if (sum && sum == y) return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm: sum and y are the same matrix");
+    const struct { uint64_t p; int64_t ld; } results[] = {{sum, lds}, {y, ldy}}, operands[] = {{x, ldx}, {residual, ldr}};
+    for (const auto& r : results)
+      for (const auto& o : operands)
+        if (int rc = check_in_place(r.p, r.ld, o.p, o.ld, rows, "rmsnorm")) return rc;
   }
   OperatorDevice d;
   if (int rc = operator_device(dev, &d)) return rc;
@@ -494,6 +505,9 @@ int sb200_rmsnorm_backward_f32(int dev, uint64_t stream, int64_t rows, int64_t c
     if (dweight && (!workspace || workspace_bytes < need))
       return set_error(SB200_ERR_INVALID_VALUE, "rmsnorm_backward: dweight needs a workspace of %llu bytes", static_cast<unsigned long long>(need));
     if (dweight && (workspace & 3)) return set_error(SB200_ERR_ALIGNMENT, "rmsnorm_backward: the workspace must be 4-byte aligned");
+    if (int rc = check_in_place(dx, lddx, sum, lds, rows, "rmsnorm_backward dx")) return rc;
+    if (int rc = check_in_place(dx, lddx, dy, lddy, rows, "rmsnorm_backward dx")) return rc;
+    if (int rc = check_in_place(dx, lddx, dsum, ldds, rows, "rmsnorm_backward dx")) return rc;
   }
   OperatorDevice d;
   if (int rc = operator_device(dev, &d)) return rc;

@@ -74,6 +74,20 @@ def test_refusals(lib, name, good, change, error):
     assert lib.sb200_last_error_string()
 
 
+APART = dict(sum=GOOD + 4096, y=GOOD + 8192)
+IN_PLACE = [("rmsnorm_f32", NORM, {}), ("rmsnorm_f32", NORM, dict(APART, sum=GOOD, lds=260)), ("rmsnorm_f32", NORM, dict(APART, y=GOOD, ldr=257)),
+            ("rmsnorm_f32", NORM, dict(APART, y=GOOD, residual=0, ldy=300)), ("gemm_mx", GEMM, dict(ldd=9)), ("gemm_mx", GEMM, dict(ldc=12)),
+            ("rmsnorm_backward_f32", BACKWARD, dict(lddx=257)), ("rmsnorm_backward_f32", BACKWARD, dict(lddy=260)),
+            ("rmsnorm_backward_f32", BACKWARD, dict(ldds=260)), ("rmsnorm_backward_f32", BACKWARD, dict(lds=260))]
+
+
+@pytest.mark.parametrize("name,good,change", IN_PLACE)
+def test_refusals_in_place(lib, name, good, change):
+    """A result that lies on an operand with other row lengths, and two results on each other."""
+    assert getattr(lib, "sb200_" + name)(0, 0, *{**good, **change}.values()) == VALUE
+    assert b"in place" in lib.sb200_last_error_string() or b"same matrix" in lib.sb200_last_error_string()
+
+
 def test_refusals_of_sizes(lib):
     a, b = C.c_uint64(), C.c_uint64()
     assert lib.sb200_mx_bytes(7, 1, 1, C.byref(a), C.byref(b)) == VALUE
