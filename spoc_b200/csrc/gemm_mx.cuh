@@ -7,12 +7,16 @@
 // of one row of D is 128 consecutive bytes at any alignment, and few rows of A make a narrow accumulator instead of idle lanes.
 //
 // Roles of a block: warps 0, 10 and 11 load B's codes, A's codes and the scale tiles with TMA into a ring of stages (a load takes a thread 80 cycles,
-// and a k-block of a narrow tile no more than its five loads: 16 x 2048 x 16384 in 8 bits took 27.2 us with one thread), warp 1 copies the scales of a stage into tensor memory
-// (p.slots in turn) and issues its MMAs, warps 2-9 run the epilogue in two groups, which take every other 32 rows of A's tile.  Beside the scales
+// and a k-block of a narrow tile no more than its five loads: 16 x 2048 x 16384 in 8 bits took 27.2 us with one thread), warp 1 copies the scales of
+// a stage into tensor memory (p.slots in turn) and issues its MMAs, warps 2-9 run the epilogue in two groups, which take every other 32 rows of A's tile.  Beside the scales
 // there is not room for two accumulators of 256 columns: they overlap, the epilogue drains the columns in common first, and the next tile's MMAs
 // begin when those are drained.  CTAS = 2: a pair of blocks on one tile of 256 columns of D; each loads its
 // own 128 rows of B, half of A's rows and all of A's scales.  A stage is 128 bytes of codes of every row: 128 values, 256 where both are e2m1;
 // e2m1 beside e4m3 is spread to a byte a value on the way into shared memory (by TMA: 16 values a 16-byte unit).
+//
+// Large products are bound by the tensor core's clock under the power cap and by the way from L2 (8192^3: 4 bits 204 to 218 us, 5.0 to 5.4 PFLOP/s; 8 bits 393
+// to 430, 2.6 to 2.8), products with few rows of A by B's bytes (16 x 16384 x 16384 in 8 bits 48.5 us, 5.7 TB/s) and small ones by latency (1 x 4096 x 4096
+// 8 by 4 bits 5.7 us).
 #pragma once
 #include <type_traits>
 

@@ -10,7 +10,8 @@
 //
 // A block a row, or a warp up to 1024 columns, the row in registers (VECS float4 a thread; thread t has columns 4 (v * threads + t)), so that x
 // and residual are read once.  Rows too long for that (32768 columns on) are read twice.  Bound by HBM: 8 bytes read, 5 written a value with
-// 8-bit codes, and by the blocks in flight: with 126 registers a thread there was one on an SM, and 8192 x 8192 took 337 us.
+// 8-bit codes, and by the blocks in flight: 8192 x 8192 with a residual to 8 bits takes 146 us (135 at the copy bandwidth), with 126 registers a thread
+// and one block an SM it took 337.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -282,8 +283,8 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
 }
 // The same for rows that a block's registers hold: groups of TG threads go from row to row, each with a ring of STAGES rows of h, dy and dsum in
 // shared memory that bulk copies fill ahead of it, so that the copies of one row run under the sums of another (8192 x 4096 131 us with a
-// row's loads in front of its sums, 90 so).  ACCESS_LANES: rows that do not all start on 16 bytes.  Copies then begin and end at the multiples of 16
-// bytes around a row; the few bytes beside it are neither used nor beyond the 16 bytes of its first and last value.
+// row's loads in front of its sums, 87 so, 83 at the copy bandwidth).  ACCESS_LANES: rows that do not all start on 16 bytes.  Copies then begin and
+// end at the multiples of 16 bytes around a row; the few bytes beside it are neither used nor beyond the 16 bytes of its first and last value.
 __device__ __forceinline__ uint32_t bulk_offset(const float* row) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) >> 2 & 3); }
 template <int TG, int G, int VECS, int STAGES, int ACCESS>
 struct BackwardRing {
