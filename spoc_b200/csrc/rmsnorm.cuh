@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS, BLOCKS) rmsnorm
 
 // The gradient: with r = 1 / sqrt(mean(h^2) + eps), n = h r and g = dy * weight,
 //   dx = dsum + r (g - n mean(g n)),   dweight = sum over the rows of dy n.
-// A block takes rows blockIdx.x, + gridDim.x, ... and keeps its part of dweight in registers (VECS = 0: in its row of the workspace); a second
-// kernel adds the parts in the order of the blocks.  h and dy are read once.  Bound by HBM: 12 bytes read and 4 written a value.
+// A block (a cluster) takes rows blockIdx.x, + gridDim.x, ... and keeps its part of dweight; a second kernel adds the parts in the order of the
+// blocks.  Bound by HBM: 12 bytes read and 4 written a value.
 struct RmsNormBackward {
   const float *h, *weight, *dy, *dsum;  // dsum may be null
   long long ldh, lddy, ldds, lddx;
@@ -191,43 +191,29 @@ struct RmsNormBackward {
   int* status;
   long long rows;
   int cols;
+  int blocks, slice;                    // of a row, where a cluster takes it
   double eps;
 };
-template <int THREADS, int VECS, int ACCESS>
-__global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNormBackward p) {
+// Rows of any length: h and dy are read twice, and the part of dweight is kept in the block's row of the workspace.
+template <int ACCESS>
+__global__ void __launch_bounds__(1024) rmsnorm_backward_kernel(const RmsNormBackward p) {
+  constexpr int THREADS = 1024, PART = ACCESS == ACCESS_VECTOR ? ACCESS_SINGLE : ACCESS;  // the workspace starts on 4 bytes
   __shared__ float2 shared[2][THREADS / 32];
   grid_launch_dependents();
   grid_dependency_wait();
   const int first = 4 * threadIdx.x;
   const float inv_cols = 1.0f / static_cast<float>(p.cols), eps = static_cast<float>(p.eps);
-  constexpr int HELD = VECS > 0 ? VECS : 1, PART = ACCESS == ACCESS_VECTOR ? ACCESS_SINGLE : ACCESS;  // the workspace starts on 4 bytes
   const long long padded = (p.cols + 127ll) / 128 * 128;
-  float4 part[HELD];
-#pragma unroll
-  for (int v = 0; v < HELD; ++v) part[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   float* const mine = p.workspace + static_cast<long long>(blockIdx.x) * p.cols;
   int turn = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
     const float *hr = p.h + row * p.ldh, *dyr = p.dy + row * p.lddy;
-    float4 h[HELD], dy[HELD];
     float2 s = make_float2(0.f, 0.f);  // of h^2 and of h * g
-    auto count = [&](const float4& a, const float4& d, const float4& w) {
+    for (long long c = first; c < padded; c += 4 * THREADS) {
+      const int col = static_cast<int>(c);
+      const float4 a = load4<ACCESS>(hr, col, p.cols), d = load4<ACCESS>(dyr, col, p.cols), w = load4<ACCESS>(p.weight, col, p.cols);
       s.x += fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w);
       s.y += fmaf(a.x, d.x * w.x, a.y * (d.y * w.y)) + fmaf(a.z, d.z * w.z, a.w * (d.w * w.w));
-    };
-    if constexpr (VECS > 0) {
-#pragma unroll
-      for (int v = 0; v < VECS; ++v) {
-        h[v] = load4<ACCESS>(hr, first + v * 4 * THREADS, p.cols);
-        dy[v] = load4<ACCESS>(dyr, first + v * 4 * THREADS, p.cols);
-      }
-#pragma unroll
-      for (int v = 0; v < VECS; ++v) count(h[v], dy[v], load4<ACCESS>(p.weight, first + v * 4 * THREADS, p.cols));
-    } else {
-      for (long long c = first; c < padded; c += 4 * THREADS) {
-        const int col = static_cast<int>(c);
-        count(load4<ACCESS>(hr, col, p.cols), load4<ACCESS>(dyr, col, p.cols), load4<ACCESS>(p.weight, col, p.cols));
-      }
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -244,7 +230,15 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
     }
     const float r = 1.0f / sqrtf(s.x * inv_cols + eps);
     const float along = s.y * inv_cols * r * r;  // mean(g n) r: what h is multiplied by
-    auto finish = [&](int col, const float4& a, const float4& d, float4& w_part) {
+    for (long long c = first; c < padded; c += 4 * THREADS) {
+      const int col = static_cast<int>(c);
+      const float4 a = load4<ACCESS>(hr, col, p.cols), d = load4<ACCESS>(dyr, col, p.cols);
+      if (p.dweight) {
+        float4 part = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row != blockIdx.x) part = load4<PART>(mine, col, p.cols);
+        store4<PART>(mine, col, p.cols,
+                     make_float4(fmaf(d.x, a.x * r, part.x), fmaf(d.y, a.y * r, part.y), fmaf(d.z, a.z * r, part.z), fmaf(d.w, a.w * r, part.w)));
+      }
       if (p.dx) {
         const float4 w = load4<ACCESS>(p.weight, col, p.cols);
         float4 o = make_float4(r * fmaf(-a.x, along, d.x * w.x), r * fmaf(-a.y, along, d.y * w.y), r * fmaf(-a.z, along, d.z * w.z),
@@ -255,36 +249,14 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_backward_kernel(const RmsNorm
         }
         store4<ACCESS>(p.dx + row * p.lddx, col, p.cols, o);
       }
-      w_part.x = fmaf(d.x, a.x * r, w_part.x);
-      w_part.y = fmaf(d.y, a.y * r, w_part.y);
-      w_part.z = fmaf(d.z, a.z * r, w_part.z);
-      w_part.w = fmaf(d.w, a.w * r, w_part.w);
-    };
-    if constexpr (VECS > 0) {
-#pragma unroll
-      for (int v = 0; v < VECS; ++v) finish(first + v * 4 * THREADS, h[v], dy[v], part[v]);
-    } else {
-      for (long long c = first; c < padded; c += 4 * THREADS) {
-        const int col = static_cast<int>(c);
-        float4 w_part = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p.dweight && row != blockIdx.x) w_part = load4<PART>(mine, col, p.cols);
-        const float4 a = load4<ACCESS>(hr, col, p.cols), d = load4<ACCESS>(dyr, col, p.cols);
-        finish(col, a, d, w_part);
-        if (p.dweight) store4<PART>(mine, col, p.cols, w_part);
-      }
-    }
-  }
-  if constexpr (VECS > 0) {
-    if (p.dweight) {
-#pragma unroll
-      for (int v = 0; v < VECS; ++v) store4<PART>(mine, first + v * 4 * THREADS, p.cols, part[v]);
     }
   }
 }
-// The same for rows that a block's registers hold: groups of TG threads go from row to row, each with a ring of STAGES rows of h, dy and dsum in
-// shared memory that bulk copies fill ahead of it, so that the copies of one row run under the sums of another (8192 x 4096 131 us with a
-// row's loads in front of its sums, 87 so, 83 at the copy bandwidth).  ACCESS_LANES: rows that do not all start on 16 bytes.  Copies then begin and
-// end at the multiples of 16 bytes around a row; the few bytes beside it are neither used nor beyond the 16 bytes of its first and last value.
+// Rows that the registers of a block, or of a cluster, hold, read once: groups of TG threads go from row to row, each with a ring of STAGES rows of
+// h, dy and dsum in shared memory that bulk copies fill ahead of it, so that the copies of one row run under the sums of another (8192 x 4096
+// 131 us with a row's loads in front of its sums, 84 so, 83 at the copy bandwidth).  ACCESS_LANES: rows that do not all start on 16 bytes.
+// Copies then begin and end at the multiples of 16 bytes around a row; the few bytes beside it are neither used nor beyond the 16 bytes of its first
+// and last value.  WIDE: a cluster of p.blocks blocks a row, each with p.slice of its columns, which send one another their sums.
 __device__ __forceinline__ uint32_t bulk_offset(const float* row) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) >> 2 & 3); }
 template <int TG, int G, int VECS, int STAGES, int ACCESS>
 struct BackwardRing {
@@ -294,35 +266,49 @@ struct BackwardRing {
   static_assert(G * kCols * 4 <= G * STAGES * kStageBytes, "the groups' parts of dweight fit the ring");
   static_assert(kArrayBytes % 16 == 0, "copies start on 16 bytes");
 };
-template <int TG, int G, int VECS, int STAGES, int BLOCKS, int ACCESS>
-__global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(const RmsNormBackward p) {
+constexpr int RMS_MAX_CLUSTER = 8;
+template <int TG, int G, int VECS, int STAGES, int ACCESS, bool WIDE>
+__global__ void __launch_bounds__(TG * G, 1) rmsnorm_backward_ring_kernel(const RmsNormBackward p) {
   using Ring = BackwardRing<TG, G, VECS, STAGES, ACCESS>;
+  static_assert(!WIDE || (G == 1 && TG >= 128), "a group of several warps");
   constexpr int PART = ACCESS == ACCESS_VECTOR ? ACCESS_SINGLE : ACCESS;  // the workspace starts on 4 bytes
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[G * STAGES];
   __shared__ float2 sums[2][G * TG / 32];
+  __shared__ float2 of_blocks[2][WIDE ? RMS_MAX_CLUSTER : 1];  // sums of the blocks of the cluster, rows in turn
+  __shared__ uint64_t sent[2];                                 // and the barriers that count them
   __shared__ int abort_word;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   const int group = threadIdx.x / TG, thread = threadIdx.x % TG, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = 4 * thread;
+  const int blocks = WIDE ? p.blocks : 1, rank = WIDE ? static_cast<int>(cluster_ctarank()) : 0;
+  const int unit = WIDE ? static_cast<int>(blockIdx.x) / blocks : static_cast<int>(blockIdx.x);
+  const int units = WIDE ? static_cast<int>(gridDim.x) / blocks : static_cast<int>(gridDim.x);
+  const int col0 = WIDE ? rank * p.slice : 0, cols = WIDE ? min(p.slice, p.cols - col0) : p.cols;
+  const float *const weight = p.weight + col0, *const h0 = p.h + col0, *const dy0 = p.dy + col0, *const dsum0 = p.dsum ? p.dsum + col0 : nullptr;
   uint8_t* mine = ring + group * STAGES * Ring::kStageBytes;
   if (threadIdx.x < G * STAGES) {
     mbar_init(smem_u32(&full[threadIdx.x]), 1);
+    if (WIDE && threadIdx.x < 2) mbar_init(smem_u32(&sent[threadIdx.x]), 1);
     mbar_fence_init();
   }
   if (threadIdx.x == 0) abort_word = 0;
   __syncthreads();
+  if (WIDE) {  // the barriers are there before another block sends
+    cluster_arrive_relaxed();
+    cluster_wait();
+  }
   grid_launch_dependents();
   grid_dependency_wait();
   const float inv_cols = 1.0f / static_cast<float>(p.cols), eps = static_cast<float>(p.eps);
-  const long long step = static_cast<long long>(gridDim.x) * G, row0 = blockIdx.x * static_cast<long long>(G) + group;
-  const uint32_t bytes = static_cast<uint32_t>(p.cols) * 4;
+  const long long step = static_cast<long long>(units) * G, row0 = unit + static_cast<long long>(units) * group;
+  const uint32_t bytes = static_cast<uint32_t>(cols) * 4;
   auto fetch = [&](int stage, long long row) {  // one thread
     const uint32_t bar = smem_u32(&full[group * STAGES + stage]), to = smem_u32(mine) + stage * Ring::kStageBytes;
     auto size = [&](const float* from) { return ((ACCESS == ACCESS_VECTOR ? 0u : bulk_offset(from)) * 4 + bytes + 15) & ~15u; };
     auto copy = [&](int array, const float* from) {
       bulk_load(to + array * Ring::kArrayBytes, ACCESS == ACCESS_VECTOR ? from : from - bulk_offset(from), size(from), bar);
     };
-    const float *h = p.h + row * p.ldh, *dy = p.dy + row * p.lddy, *ds = p.dsum + row * p.ldds;
+    const float *h = h0 + row * p.ldh, *dy = dy0 + row * p.lddy, *ds = dsum0 + row * p.ldds;
     mbar_arrive_expect_tx(bar, size(h) + size(dy) + (p.dsum ? size(ds) : 0));
     copy(0, h);
     copy(1, dy);
@@ -336,15 +322,15 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
   float4 w[VECS], part[VECS];
 #pragma unroll
   for (int v = 0; v < VECS; ++v) {
-    w[v] = load4<ACCESS>(p.weight, first + v * 4 * TG, p.cols);
+    w[v] = load4<ACCESS>(weight, first + v * 4 * TG, cols);
     part[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   int stage = 0, turn = 0;
-  uint32_t phase = 0;
+  uint32_t phase = 0, sent_phase = 0;
   bool ok = true;
-  for (long long row = row0; row < p.rows; row += step, turn ^= 1) {
+  for (long long row = row0; row < p.rows; row += step) {
     const uint8_t* from = mine + stage * Ring::kStageBytes;
-    ok = mbar_wait_bounded(smem_u32(&full[group * STAGES + stage]), phase, &abort_word);
+    ok = mbar_wait_bounded(smem_u32(&full[group * STAGES + stage]), phase, &abort_word) && ok;
     float4 h[VECS], dy[VECS], ds[VECS];
     float2 s = make_float2(0.f, 0.f);  // of h^2 and of h * g
 #pragma unroll
@@ -353,39 +339,61 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
       const float* const at = reinterpret_cast<const float*>(from);
       h[v] = dy[v] = ds[v] = make_float4(0.f, 0.f, 0.f, 0.f);
       if constexpr (ACCESS == ACCESS_VECTOR) {
-        if (col < p.cols) {
+        if (col < cols) {
           h[v] = *reinterpret_cast<const float4*>(at + col);
           dy[v] = *reinterpret_cast<const float4*>(at + Ring::kArrayBytes / 4 + col);
           if (p.dsum) ds[v] = *reinterpret_cast<const float4*>(at + 2 * (Ring::kArrayBytes / 4) + col);
         }
       } else {
-        h[v] = load4<ACCESS>(at + bulk_offset(p.h + row * p.ldh), col, p.cols);
-        dy[v] = load4<ACCESS>(at + Ring::kArrayBytes / 4 + bulk_offset(p.dy + row * p.lddy), col, p.cols);
-        if (p.dsum) ds[v] = load4<ACCESS>(at + 2 * (Ring::kArrayBytes / 4) + bulk_offset(p.dsum + row * p.ldds), col, p.cols);
+        h[v] = load4<ACCESS>(at + bulk_offset(h0 + row * p.ldh), col, cols);
+        dy[v] = load4<ACCESS>(at + Ring::kArrayBytes / 4 + bulk_offset(dy0 + row * p.lddy), col, cols);
+        if (p.dsum) ds[v] = load4<ACCESS>(at + 2 * (Ring::kArrayBytes / 4) + bulk_offset(dsum0 + row * p.ldds), col, cols);
       }
       const float4 &a = h[v], &d = dy[v];
       s.x += fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w);
       s.y += fmaf(a.x, d.x * w[v].x, a.y * (d.y * w[v].y)) + fmaf(a.z, d.z * w[v].z, a.w * (d.w * w[v].w));
     }
+    auto over_warp = [](float2& x) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
-      s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
-    }
+      for (int o = 16; o; o >>= 1) {
+        x.x += __shfl_xor_sync(0xffffffffu, x.x, o);
+        x.y += __shfl_xor_sync(0xffffffffu, x.y, o);
+      }
+    };
+    over_warp(s);
     if (TG > 32) {
       if (lane == 0) sums[turn][warp] = s;
       ok = barrier_all(1 + group, TG, ok);  // the group has read the stage; all of it goes on, or none
+    } else {
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (!ok) break;
+    if constexpr (WIDE) {
+      // A block sends its sums of the next row when all its threads have read those of this one, so that those of the row after that may be
+      // written over them.  Who gives up here does so at the next row, with its whole block.
+      if (warp == 3) {
+        s = lane < TG / 32 ? sums[turn][lane] : make_float2(0.f, 0.f);
+        over_warp(s);
+        const uint32_t bar = smem_u32(&sent[turn]);
+        if (lane == 0) mbar_arrive_expect_tx(bar, blocks * 8);
+        if (lane < blocks) st_async_f32x2(map_to_cta(smem_u32(&of_blocks[turn][rank]), lane), s, map_to_cta(bar, lane));
+      }
+      ok = mbar_wait_cluster(smem_u32(&sent[turn]), sent_phase, &abort_word);
+      s = make_float2(0.f, 0.f);
+      for (int k = 0; k < blocks; ++k) {
+        s.x += of_blocks[turn][k].x;
+        s.y += of_blocks[turn][k].y;
+      }
+      sent_phase ^= turn;
+    } else if (TG > 32) {
       s = make_float2(0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < TG / 32; ++k) {
         s.x += sums[turn][group * (TG / 32) + k].x;
         s.y += sums[turn][group * (TG / 32) + k].y;
       }
-    } else {
-      ok = __all_sync(0xffffffffu, ok);
     }
-    if (!ok) break;
-    if (thread == 0 && row + STAGES * step < p.rows) fetch(stage, row + STAGES * step);
+    turn ^= 1;
     const float r = 1.0f / sqrtf(s.x * inv_cols + eps);
     const float along = s.y * inv_cols * r * r;  // mean(g n) r: what h is multiplied by
 #pragma unroll
@@ -394,27 +402,34 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
       if (p.dx) {
         const float4 o = make_float4(r * fmaf(-a.x, along, d.x * w[v].x) + ds[v].x, r * fmaf(-a.y, along, d.y * w[v].y) + ds[v].y,
                                      r * fmaf(-a.z, along, d.z * w[v].z) + ds[v].z, r * fmaf(-a.w, along, d.w * w[v].w) + ds[v].w);
-        store4<ACCESS>(p.dx + row * p.lddx, first + v * 4 * TG, p.cols, o);
+        store4<ACCESS>(p.dx + col0 + row * p.lddx, first + v * 4 * TG, cols, o);
       }
       part[v].x = fmaf(d.x, a.x * r, part[v].x);
       part[v].y = fmaf(d.y, a.y * r, part[v].y);
       part[v].z = fmaf(d.z, a.z * r, part[v].z);
       part[v].w = fmaf(d.w, a.w * r, part[v].w);
     }
+    // behind the row's stores: in front of them the copies hold those up (8192 x 8191 199 us, 160 so)
+    if (thread == 0 && row + STAGES * step < p.rows) fetch(stage, row + STAGES * step);
     if (++stage == STAGES) {
       stage = 0;
       phase ^= 1u;
     }
   }
   if (!ok) {
-    if (lane == 0) atomicCAS(p.status, 0, 0x3100 | group);
+    atomicCAS(p.status, 0, 0x3100 | group);
     wait_for_copies();
   }
+  if (WIDE) {  // no block retires while another can still send to it
+    __syncwarp();
+    cluster_arrive_relaxed();
+    cluster_wait();
+  }
   if (!p.dweight) return;
-  float* const to = p.workspace + static_cast<long long>(blockIdx.x) * p.cols;
+  float* const to = p.workspace + static_cast<long long>(unit) * p.cols + col0;
   if (G == 1) {
 #pragma unroll
-    for (int v = 0; v < VECS; ++v) store4<PART>(to, first + v * 4 * TG, p.cols, part[v]);
+    for (int v = 0; v < VECS; ++v) store4<PART>(to, first + v * 4 * TG, cols, part[v]);
     return;
   }
   __syncthreads();  // no copy is in flight: every group has waited for all that it asked for
@@ -422,7 +437,7 @@ __global__ void __launch_bounds__(TG * G, BLOCKS) rmsnorm_backward_ring_kernel(c
 #pragma unroll
   for (int v = 0; v < VECS; ++v) store4<ACCESS>(shared_part + group * Ring::kCols, first + v * 4 * TG, Ring::kCols, part[v]);
   __syncthreads();
-  for (int c = threadIdx.x; c < p.cols; c += TG * G) {
+  for (int c = threadIdx.x; c < cols; c += TG * G) {
     float s = 0.0f;
 #pragma unroll
     for (int g = 0; g < G; ++g) s += shared_part[g * Ring::kCols + c];

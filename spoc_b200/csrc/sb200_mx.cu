@@ -118,48 +118,47 @@ int launch_rmsnorm(int sm_count, cudaStream_t st, const RmsNorm& p) {
 
 int64_t dweight_parts(int64_t rows) { return std::min<int64_t>(rows, SB200_RMSNORM_MAX_PARTS); }
 
-template <int TG, int G, int VECS, int STAGES, int BLOCKS, int ACCESS>
-int launch_backward_ring(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, unsigned* grid) {
+// As many blocks, or clusters, as are resident at once.
+template <int TG, int G, int VECS, int STAGES, int ACCESS, bool WIDE = false>
+int launch_backward_ring(const OperatorDevice& d, cudaStream_t st, RmsNormBackward p, unsigned* parts) {
   using Ring = BackwardRing<TG, G, VECS, STAGES, ACCESS>;
-  auto kernel = rmsnorm_backward_ring_kernel<TG, G, VECS, STAGES, BLOCKS, ACCESS>;
+  auto kernel = rmsnorm_backward_ring_kernel<TG, G, VECS, STAGES, ACCESS, WIDE>;
   static std::atomic<bool> ready[kMaxDevices];
   if (!ready[d.index].load()) {
     CU_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring::kBytes));
     ready[d.index].store(true);
   }
-  *grid = static_cast<unsigned>(std::min<int64_t>((p.rows + G - 1) / G, std::min(d.sm_count * BLOCKS, SB200_RMSNORM_MAX_PARTS)));
+  p.blocks = WIDE ? (p.cols + Ring::kCols - 1) / Ring::kCols : 1;
+  p.slice = WIDE ? ((p.cols + p.blocks - 1) / p.blocks + 3) / 4 * 4 : p.cols;  // slices of rows on 16 bytes start there, too
+  const int64_t units = std::max<int64_t>(1, WIDE ? cluster_capacity(p.blocks, d.sm_count) : d.sm_count);
+  *parts = static_cast<unsigned>(std::min(units, dweight_parts(p.rows)));
   operator_waits(d.index);
-  CU_TRY(launch_pdl(kernel, dim3(*grid), dim3(TG * G), Ring::kBytes, st, 1, p));
+  CU_TRY(launch_pdl(kernel, dim3(*parts * p.blocks), dim3(TG * G), Ring::kBytes, st, p.blocks, p));
   return operator_launched("rmsnorm_backward_ring_kernel");
 }
 template <int ACCESS>
-int launch_backward_rings(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, unsigned* grid) {
+int launch_backward(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, unsigned* parts) {
   const int cols = p.cols;
-  if (cols <= 128) return launch_backward_ring<32, 8, 1, 4, 3, ACCESS>(d, st, p, grid);
-  if (cols <= 512) return launch_backward_ring<128, 2, 1, 5, 3, ACCESS>(d, st, p, grid);
-  if (cols <= 1024) return launch_backward_ring<256, 1, 1, 5, 3, ACCESS>(d, st, p, grid);
-  if (cols <= 2048) return launch_backward_ring<256, 1, 2, 3, 3, ACCESS>(d, st, p, grid);
-  if (cols <= 4096) return launch_backward_ring<512, 1, 2, 2, 2, ACCESS>(d, st, p, grid);
-  return launch_backward_ring<1024, 1, 2, 2, 1, ACCESS>(d, st, p, grid);
-}
-template <bool VEC>
-int launch_backward_rows(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, unsigned* grid) {
-  *grid = static_cast<unsigned>(std::min<int64_t>(dweight_parts(p.rows), static_cast<int64_t>(d.sm_count) * 2));
-#define SB200_NORM(THREADS, VECS) CU_TRY(launch_pdl(rmsnorm_backward_kernel<THREADS, VECS, VEC ? ACCESS_VECTOR : ACCESS_LANES>, dim3(*grid), dim3(THREADS), 0, st, 1, p))
-  const int64_t cols = p.cols;
-  if (cols <= 16384) SB200_NORM(512, 8);
-  else SB200_NORM(1024, 0);
-#undef SB200_NORM
+  // A block an SM with a ring of 196 KB.  Groups of the fewest warps that hold a row in four float4 a thread: with twice the threads and two float4
+  // 4096 x 16384 took 178 us instead of 158 (and 255 without a cluster), 8192 x 8191 183 instead of 160.
+  if (cols <= 128) return launch_backward_ring<32, 32, 1, 4, ACCESS>(d, st, p, parts);
+  if (cols <= 256) return launch_backward_ring<32, 16, 2, 4, ACCESS>(d, st, p, parts);
+  if (cols <= 512) return launch_backward_ring<32, 8, 4, 4, ACCESS>(d, st, p, parts);
+  if (cols <= 1024) return launch_backward_ring<64, 4, 4, 4, ACCESS>(d, st, p, parts);
+  if (cols <= 2048) return launch_backward_ring<128, 4, 4, 2, ACCESS>(d, st, p, parts);
+  if (cols <= 4096) return launch_backward_ring<256, 2, 4, 2, ACCESS>(d, st, p, parts);
+  if (cols <= 8192) return launch_backward_ring<512, 1, 4, 2, ACCESS>(d, st, p, parts);
+  if (cols <= 8192 * RMS_MAX_CLUSTER) return launch_backward_ring<512, 1, 4, 2, ACCESS, true>(d, st, p, parts);
+  *parts = static_cast<unsigned>(std::min<int64_t>(dweight_parts(p.rows), static_cast<int64_t>(d.sm_count) * 2));
+  CU_TRY(launch_pdl(rmsnorm_backward_kernel<ACCESS>, dim3(*parts), dim3(1024), 0, st, 1, p));
   return operator_launched("rmsnorm_backward_kernel");
 }
 int launch_rmsnorm_backward(const OperatorDevice& d, cudaStream_t st, const RmsNormBackward& p, bool vec) {
-  unsigned grid = 0;
-  int rc;
-  if (p.cols <= 8192) rc = vec ? launch_backward_rings<ACCESS_VECTOR>(d, st, p, &grid) : launch_backward_rings<ACCESS_LANES>(d, st, p, &grid);
-  else rc = vec ? launch_backward_rows<true>(d, st, p, &grid) : launch_backward_rows<false>(d, st, p, &grid);
+  unsigned parts = 0;
+  const int rc = vec ? launch_backward<ACCESS_VECTOR>(d, st, p, &parts) : launch_backward<ACCESS_LANES>(d, st, p, &parts);
   if (rc || !p.dweight) return rc;
   CU_TRY(launch_pdl(rmsnorm_dweight_kernel, dim3(grid_for(p.cols, 32, 1 << 20)), dim3(256), 0, st, 1, static_cast<const float*>(p.workspace),
-                    static_cast<int>(grid), p.dweight, static_cast<long long>(p.cols)));
+                    static_cast<int>(parts), p.dweight, static_cast<long long>(p.cols)));
   return operator_launched("rmsnorm_dweight_kernel");
 }
 

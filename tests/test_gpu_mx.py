@@ -412,6 +412,16 @@ def test_norm_backward_rows(keep, device, rows, cols):
     check_backward(run_backward(keep, device, h, w, dy, ds, 1e-5, in_place="dsum" if rows % 2 else None), h, w, dy, ds, 1e-5)
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 8193), (300, 8196), (150, 12001), (75, 16384), (2, 16385), (180, 20004), (101, 24577), (77, 40000), (43, 49155),
+                                       (31, 65535), (60, 65536), (3, 65537)])
+def test_norm_backward_wide(keep, device, rows, cols):
+    """Rows of two to eight blocks, up to five for a cluster, and those that no cluster takes."""
+    rng = np.random.default_rng(cols)
+    h, w = loud(rng, rows, cols), rng.normal(size=cols).astype(np.float32)
+    dy, ds = loud(rng, rows, cols), loud(rng, rows, cols) if rows % 2 else None
+    check_backward(run_backward(keep, device, h, w, dy, ds, 1e-5, 3 if rows % 5 == 0 else 0, 0, "dy" if rows % 3 == 0 else None), h, w, dy, ds, 1e-5)
+
+
 def test_norm_backward_against_differences(keep, device):
     """The loss sum(c * y) changes by dx and dweight, to a difference's error: central differences of the formula in 64 bits."""
     rng = np.random.default_rng(8)
