@@ -47,10 +47,18 @@ __device__ __forceinline__ float mx_scale_value(uint32_t scale) {
   return __uint_as_float(scale == 255u ? 0x7fc00000u : scale == 0u ? 0x00400000u : scale << 23);
 }
 
+// Two products with one instruction, rounded as two are.
+__device__ __forceinline__ float2 multiply2(float2 a, float2 b) {
+  float2 v;
+  asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}"
+      : "=f"(v.x), "=f"(v.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return v;
+}
 // Four values, scaled, to four codes: 32 bits of e4m3, or 16 of e2m1.
 template <bool FP4>
 __device__ __forceinline__ uint32_t mx_codes4(float4 v, float factor) {
-  const float2 a = make_float2(v.x * factor, v.y * factor), b = make_float2(v.z * factor, v.w * factor);
+  const float2 f = make_float2(factor, factor), a = multiply2(make_float2(v.x, v.y), f), b = multiply2(make_float2(v.z, v.w), f);
   if constexpr (FP4)
     return static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(a, __NV_E2M1, cudaRoundNearest)) |
            static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(b, __NV_E2M1, cudaRoundNearest)) << 8;

@@ -69,11 +69,11 @@ struct RmsRow {
   double mean;      // of the squares, plus eps
   float unit;       // 1, or a power of two that brings values of a mean far from 1 near to it
   float scale;      // 1 / (unit * sqrt(mean)), nearly
-  float* y;         // each result's row, or null
-  uint8_t *codes, *scales;
+  float* y;         // the result's row, or null
+  uint8_t *codes, *scales;  // of the warp's first chunk
 };
 template <int FORMAT>
-__device__ __forceinline__ RmsRow rmsnorm_row(const RmsNorm& p, long long row, double sum) {
+__device__ __forceinline__ RmsRow rmsnorm_row(const RmsNorm& p, long long row, int first_chunk, double sum) {
   RmsRow r;
   r.mean = fma(sum, p.inv_cols, p.eps);
   const int half = (static_cast<int>(__double2hiint(r.mean) >> 20 & 0x7ff) - 1023) / 2;
@@ -82,38 +82,40 @@ __device__ __forceinline__ RmsRow rmsnorm_row(const RmsNorm& p, long long row, d
   const float m = static_cast<float>(r.mean * r.unit * r.unit), s = rsqrtf(m), e = fmaf(-m * s, s, 1.0f);
   r.scale = s > 0.0f ? fmaf(0.5f * s, e, s) : s;  // of an infinite mean 0
   r.y = p.y ? p.y + row * p.ldy : nullptr;
-  r.codes = p.codes + row * p.chunks * (FORMAT == 4 ? 64 : 128);
-  r.scales = p.scales + mx_scale_offset(row, 0, p.chunks);
+  r.codes = p.codes + (row * p.chunks + first_chunk) * (FORMAT == 4 ? 64 : 128);
+  r.scales = p.scales + mx_scale_offset(row, first_chunk, p.chunks);
   return r;
 }
-// Four values of the normed row from column `col` on.  FORMAT: 0 float32 only, 4, 8.
+// Four values of the normed row from column `col` on, `ahead` chunks behind the warp's first.  FORMAT: 0 float32 only, 4, 8.
 template <int FORMAT, int ACCESS>
-__device__ __forceinline__ void rmsnorm_emit(const RmsNorm& p, const RmsRow& row, int col, const float4& h, int lane) {
-  const float s = row.scale;
+__device__ __forceinline__ void rmsnorm_emit(const RmsNorm& p, const RmsRow& row, int col, int ahead, const float4& h, int lane) {
   const float4 w = load4<ACCESS>(p.weight, col, p.cols);
   float4 y = h;
   if (row.unit != 1.0f) y = make_float4(h.x * row.unit, h.y * row.unit, h.z * row.unit, h.w * row.unit);
-  y = make_float4(y.x * s * w.x, y.y * s * w.y, y.z * s * w.z, y.w * s * w.w);
+  const float2 s = make_float2(row.scale, row.scale);
+  const float2 y01 = multiply2(multiply2(make_float2(y.x, y.y), s), make_float2(w.x, w.y)), y23 = multiply2(multiply2(make_float2(y.z, y.w), s), make_float2(w.z, w.w));
+  y = make_float4(y01.x, y01.y, y23.x, y23.y);
   if (row.y) store4<ACCESS>(row.y, col, p.cols, y);
   if constexpr (FORMAT != 0) {
     constexpr bool FP4 = FORMAT == 4;
-    const int chunk = col / MX_CHUNK;  // the same in a whole warp
-    if (chunk >= p.chunks) return;
-    uint8_t* codes = row.codes + static_cast<long long>(chunk) * MxFormat<FP4>::kChunkBytes;
-    uint8_t* scales = row.scales + static_cast<long long>(chunk) * MX_TILE_BYTES;
+    if (col >> 7 >= p.chunks) return;  // the same in a whole warp
+    uint8_t* codes = row.codes + static_cast<long long>(ahead) * MxFormat<FP4>::kChunkBytes;
+    uint8_t* scales = row.scales + static_cast<long long>(ahead) * MX_TILE_BYTES;
     const uint32_t m = largest_of_block(y), block_scale = mx_scale_of<FP4>(m);
     const float f = mx_factor(block_scale), top = __uint_as_float(m);
     const uint32_t low = mx_codes4<FP4>(y, f * (1.0f - RMS_DOUBT)), high = mx_codes4<FP4>(y, f * (1.0f + RMS_DOUBT));
     // The estimate holds for weights below 2^40 and a largest value between 2^-60 and 2^100: products that fall below float32's range then lose
     // nothing that a code shows.  A block of zeros holds too, where h is zero.
-    bool again = low != high || !(fmaxf(fmaxf(fabsf(w.x), fabsf(w.y)), fmaxf(fabsf(w.z), fabsf(w.w))) < 1.09951163e12f);
-    again = again || (m == 0 ? (abs_bits(h.x) | abs_bits(h.y) | abs_bits(h.z) | abs_bits(h.w)) != 0
-                             : m - (67u << 23) >= 160u << 23 ||
-                                   ((__float_as_uint(top * (1.0f - RMS_DOUBT)) ^ __float_as_uint(top * (1.0f + RMS_DOUBT))) >> 23) != 0);
-    if (__any_sync(0xffffffffu, again))
-      rmsnorm_chunk_exact<FP4>(h, w, row.mean, codes, scales, lane);
-    else
-      mx_store_codes<FP4>(low, block_scale, codes, scales, lane);
+    bool again = low != high || !(fmaxf(fmaxf(fabsf(w.x), fabsf(w.y)), fmaxf(fabsf(w.z), fabsf(w.w))) < 1.09951163e12f) || m - (67u << 23) >= 160u << 23 ||
+                 ((__float_as_uint(top * (1.0f - RMS_DOUBT)) ^ __float_as_uint(top * (1.0f + RMS_DOUBT))) >> 23) != 0;
+    if (__any_sync(0xffffffffu, again)) {
+      if (m == 0 && low == high) again = (abs_bits(h.x) | abs_bits(h.y) | abs_bits(h.z) | abs_bits(h.w)) != 0;
+      if (__any_sync(0xffffffffu, again)) {
+        rmsnorm_chunk_exact<FP4>(h, w, row.mean, codes, scales, lane);
+        return;
+      }
+    }
+    mx_store_codes<FP4>(low, block_scale, codes, scales, lane);
   }
 }
 template <int ACCESS>
@@ -129,12 +131,25 @@ __device__ __forceinline__ double squares(const float4& h) {
   return fma(static_cast<double>(h.x), static_cast<double>(h.x), static_cast<double>(h.y) * h.y) +
          fma(static_cast<double>(h.z), static_cast<double>(h.z), static_cast<double>(h.w) * h.w);
 }
+// The values of a chunk side by side in the lanes (ACCESS_LANES), turned to four in a row a lane.
+__device__ __forceinline__ float4 turned(const float4& v, float4* chunk, int lane) {
+  float* const flat = reinterpret_cast<float*>(chunk);
+  __syncwarp();  // what was there before is read
+  flat[lane] = v.x;
+  flat[lane + 32] = v.y;
+  flat[lane + 64] = v.z;
+  flat[lane + 96] = v.w;
+  __syncwarp();
+  return chunk[lane];
+}
 // THREADS: of a row; 32: a block has four rows.  VECS = 0: rows of any length, read twice (h may be x or residual itself: then the second
 // reading takes h, which was stored).
 template <int FORMAT, int THREADS, int VECS, int ACCESS, int BLOCKS>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS, BLOCKS) rmsnorm_kernel(const RmsNorm p) {
   constexpr int ROWS = THREADS == 32 ? 4 : 1;
+  constexpr int GLOBAL = VECS > 0 && ACCESS == ACCESS_SINGLE ? ACCESS_LANES : ACCESS;  // of x, residual and h
   __shared__ double shared[2][THREADS / 32];
+  __shared__ float4 turn_of[GLOBAL == ACCESS ? 1 : THREADS == 32 ? 128 : THREADS];
   grid_launch_dependents();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, thread = THREADS == 32 ? lane : threadIdx.x, first = 4 * thread;
@@ -149,18 +164,22 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS, BLOCKS) rmsnorm
     if constexpr (VECS > 0) {
       float4 h[VECS];
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) h[v] = rmsnorm_input<ACCESS>(p, row, first + v * 4 * THREADS);
+      for (int v = 0; v < VECS; ++v) h[v] = rmsnorm_input<GLOBAL>(p, row, first + v * 4 * THREADS);
       double s = 0.0;
 #pragma unroll
       for (int v = 0; v < VECS; ++v) s += squares(h[v]);
       if (p.h) {
         float* to = p.h + row * p.ldh;
 #pragma unroll
-        for (int v = 0; v < VECS; ++v) store4<ACCESS>(to, first + v * 4 * THREADS, p.cols, h[v]);
+        for (int v = 0; v < VECS; ++v) store4<GLOBAL>(to, first + v * 4 * THREADS, p.cols, h[v]);
       }
-      const RmsRow r = rmsnorm_row<FORMAT>(p, row, block_sum<THREADS>(s, shared[turn]));
+      if constexpr (GLOBAL != ACCESS) {
 #pragma unroll
-      for (int v = 0; v < VECS; ++v) rmsnorm_emit<FORMAT, ACCESS>(p, r, first + v * 4 * THREADS, h[v], lane);
+        for (int v = 0; v < VECS; ++v) h[v] = turned(h[v], turn_of + (threadIdx.x & ~31), lane);
+      }
+      const RmsRow r = rmsnorm_row<FORMAT>(p, row, first >> 7, block_sum<THREADS>(s, shared[turn]));
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) rmsnorm_emit<FORMAT, ACCESS>(p, r, first + v * 4 * THREADS, v * (THREADS / 32), h[v], lane);
     } else {
       const long long padded = static_cast<long long>(p.chunks) * MX_CHUNK;
       double s = 0.0;
@@ -170,11 +189,11 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS, BLOCKS) rmsnorm
         s += squares(h);
         if (p.h) store4<ACCESS>(p.h + row * p.ldh, col, p.cols, h);
       }
-      const RmsRow r = rmsnorm_row<FORMAT>(p, row, block_sum<THREADS>(s, shared[turn]));
+      const RmsRow r = rmsnorm_row<FORMAT>(p, row, first >> 7, block_sum<THREADS>(s, shared[turn]));
       for (long long c = first; c < padded; c += 4 * THREADS) {
         const int col = static_cast<int>(c);
         const float4 h = p.h ? load4<ACCESS>(p.h + row * p.ldh, col, p.cols) : rmsnorm_input<ACCESS>(p, row, col);
-        rmsnorm_emit<FORMAT, ACCESS>(p, r, col, h, lane);
+        rmsnorm_emit<FORMAT, ACCESS>(p, r, col, (col - first) >> 7, h, lane);
       }
     }
   }
