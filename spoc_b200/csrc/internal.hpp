@@ -31,25 +31,37 @@ int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void*
 
 // Launches a kernel with programmatic stream serialization: it may set itself up while the kernel before it in the stream
 // still runs.  Every kernel launched this way passes griddepcontrol.wait before it touches global memory.  The launch call
-// itself is cheaper too (2.3 against 2.8 us).
+// itself is cheaper too (2.3 against 2.8 us).  shared_percent: the share of an SM's L1 that should be shared memory, -1 as the driver sees fit.
 template <class... Params, class... Args>
-cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, Args&&... args) {
+cudaError_t launch_pdl_sharing(int shared_percent, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, Args&&... args) {
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[3];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
+  cfg.numAttrs = 1;
+  if (cluster > 1) {
+    cudaLaunchAttribute& a = attr[cfg.numAttrs++];
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = static_cast<unsigned>(cluster);
+    a.val.clusterDim.y = 1;
+    a.val.clusterDim.z = 1;
+  }
+  if (shared_percent >= 0) {
+    cudaLaunchAttribute& a = attr[cfg.numAttrs++];
+    a.id = cudaLaunchAttributePreferredSharedMemoryCarveout;
+    a.val.sharedMemCarveout = static_cast<unsigned>(shared_percent);
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+template <class... Params, class... Args>
+cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, Args&&... args) {
+  return launch_pdl_sharing(-1, kernel, grid, block, smem, st, cluster, std::forward<Args>(args)...);
 }
 
 // Clusters of `blocks` (at most 8) blocks that are resident at once when every block has an SM to itself.  A cluster lies within a

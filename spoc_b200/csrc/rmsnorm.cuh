@@ -10,7 +10,7 @@
 //
 // A block a row, or a warp up to 1024 columns, the row in registers (VECS float4 a thread; thread t has columns 4 (v * threads + t)), so that x
 // and residual are read once.  Rows too long for that (32768 columns on) are read twice.  Bound by HBM: 8 bytes read, 5 written a value with
-// 8-bit codes, and by the blocks in flight: 8192 x 8192 with a residual to 8 bits takes 146 us (135 at the copy bandwidth), with 126 registers a thread
+// 8-bit codes, and by the blocks in flight: 8192 x 8192 with a residual to 8 bits takes 142 us (135 at the copy bandwidth), with 126 registers a thread
 // and one block an SM it took 337.
 #pragma once
 #include <cuda_runtime.h>
@@ -130,17 +130,6 @@ __device__ __forceinline__ float4 rmsnorm_input(const RmsNorm& p, long long row,
 __device__ __forceinline__ double squares(const float4& h) {
   return fma(static_cast<double>(h.x), static_cast<double>(h.x), static_cast<double>(h.y) * h.y) +
          fma(static_cast<double>(h.z), static_cast<double>(h.z), static_cast<double>(h.w) * h.w);
-}
-// The values of a chunk side by side in the lanes (ACCESS_LANES), turned to four in a row a lane.
-__device__ __forceinline__ float4 turned(const float4& v, float4* chunk, int lane) {
-  float* const flat = reinterpret_cast<float*>(chunk);
-  __syncwarp();  // what was there before is read
-  flat[lane] = v.x;
-  flat[lane + 32] = v.y;
-  flat[lane + 64] = v.z;
-  flat[lane + 96] = v.w;
-  __syncwarp();
-  return chunk[lane];
 }
 // THREADS: of a row; 32: a block has four rows.  VECS = 0: rows of any length, read twice (h may be x or residual itself: then the second
 // reading takes h, which was stored).
