@@ -451,9 +451,8 @@ SB200_API int sb200_rmsnorm_f32(int dev, uint64_t stream, int64_t rows, int64_t 
  *   dx = dsum + r * (g - n * mean(g * n))  (the gradient of x and of residual),  dweight = sum over the rows of dy * n,
  * dsum the gradient that reaches `sum` from elsewhere (may be 0).  dx or dweight may be 0; dx may be dy, dsum or sum at the same leading
  * dimension.  dweight needs a workspace of sb200_rmsnorm_workspace_bytes: min(rows, 512) * cols * 4; calls that may run at the same
- * time need one each.  Results do not depend on timing.  Sums are float32, those of the squares among them: values of `sum` beyond 1e18, and
- * rows that lie below 1e-18 with an eps that small, are out of their range (the norm itself takes them).  Of no rows dweight is zero: a
- * memset, where the other calls are kernel launches alone. */
+ * time need one each.  Results do not depend on timing.  r is float32: rows whose sqrt(mean(sum^2) + eps) lies below 1e-37 or above 1e37 are
+ * out of its range (the norm itself takes them).  Of no rows dweight is zero: a memset, where the other calls are kernel launches alone. */
 #define SB200_RMSNORM_MAX_PARTS 512
 SB200_API int sb200_rmsnorm_workspace_bytes(int64_t rows, int64_t cols, uint64_t *bytes);
 SB200_API int sb200_rmsnorm_backward_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint64_t sum, int64_t lds, uint64_t weight,

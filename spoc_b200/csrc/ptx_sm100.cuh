@@ -304,10 +304,15 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
   return v;
 }
-// Two floats into the shared memory of a block of the cluster, completing their 8 bytes on a barrier of that block (addresses from map_to_cta): who
+// Two numbers into the shared memory of a block of the cluster, completing their bytes on a barrier of that block (addresses from map_to_cta): who
 // has waited for the barrier sees them.
-__device__ __forceinline__ void st_async_f32x2(uint32_t cluster_addr, float2 v, uint32_t bar_cluster_addr) {
+__device__ __forceinline__ void st_async_pair(uint32_t cluster_addr, float2 v, uint32_t bar_cluster_addr) {
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(cluster_addr), "f"(v.x), "f"(v.y),
+               "r"(bar_cluster_addr)
+               : "memory");
+}
+__device__ __forceinline__ void st_async_pair(uint32_t cluster_addr, double2 v, uint32_t bar_cluster_addr) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];" ::"r"(cluster_addr), "d"(v.x), "d"(v.y),
                "r"(bar_cluster_addr)
                : "memory");
 }

@@ -64,6 +64,20 @@ __device__ __noinline__ void rmsnorm_chunk_exact(float4 h, float4 w, double mean
   mx_store_chunk<FP4>(y, mx_scale_of<FP4>(largest_of_block(y)), codes, scales, lane);
 }
 
+// 1 / sqrt(m) of a finite m: rsqrtf is two units in the last place off; a step of Newton's leaves the error of its own two roundings.
+__device__ __forceinline__ float refined_root(float m) {
+  const float s = rsqrtf(m);
+  return fmaf(0.5f * s, fmaf(-m * s, s, 1.0f), s);
+}
+// 1 / sqrt(mean) is the result times *unit, which is 1, or a power of two that brings a mean far from 1 near to it.
+__device__ __forceinline__ float inverse_root(double mean, float* unit) {
+  const int half = (static_cast<int>(__double2hiint(mean) >> 20 & 0x7ff) - 1023) / 2;
+  const float u = abs(half) < 45 ? 1.0f : __uint_as_float(static_cast<uint32_t>(min(max(127 - half, 1), 254)) << 23);
+  const float m = static_cast<float>(mean * u * u), s = refined_root(m);
+  *unit = u;
+  return m < INFINITY ? s : rsqrtf(m);  // of an infinite mean 0
+}
+
 // What a row's results need.
 struct RmsRow {
   double mean;      // of the squares, plus eps
@@ -76,11 +90,7 @@ template <int FORMAT>
 __device__ __forceinline__ RmsRow rmsnorm_row(const RmsNorm& p, long long row, int first_chunk, double sum) {
   RmsRow r;
   r.mean = fma(sum, p.inv_cols, p.eps);
-  const int half = (static_cast<int>(__double2hiint(r.mean) >> 20 & 0x7ff) - 1023) / 2;
-  r.unit = abs(half) < 45 ? 1.0f : __uint_as_float(static_cast<uint32_t>(min(max(127 - half, 1), 254)) << 23);
-  // rsqrtf is two units in the last place off; a step of Newton's leaves the error of its own two roundings
-  const float m = static_cast<float>(r.mean * r.unit * r.unit), s = rsqrtf(m), e = fmaf(-m * s, s, 1.0f);
-  r.scale = s > 0.0f ? fmaf(0.5f * s, e, s) : s;  // of an infinite mean 0
+  r.scale = inverse_root(r.mean, &r.unit);
   r.y = p.y ? p.y + row * p.ldy : nullptr;
   r.codes = p.codes + (row * p.chunks + first_chunk) * (FORMAT == 4 ? 64 : 128);
   r.scales = p.scales + mx_scale_offset(row, first_chunk, p.chunks);
@@ -200,62 +210,102 @@ struct RmsNormBackward {
   long long rows;
   int cols;
   int blocks, slice;                    // of a row, where a cluster takes it
-  double eps;
+  float least;                          // sums of squares below it are too small for float32
+  double inv_cols, eps;
 };
-// Rows of any length: h and dy are read twice, and the part of dweight is kept in the block's row of the workspace.
+// A row's two sums, of h^2 and of h g, are float32 where they hold: squares of values past 2^64 / sqrt(cols) are infinite, and r zero, and squares
+// below 2^-126 lose bits, which nothing shows beside an eps of 2^-80 or a sum of that.  Other rows are summed again in 64 bits; doing so for every row
+// took 8192 x 4095 from 87 to 106 us and 16384 x 256 from 14.5 to 15.6.
+constexpr double RMS_LEAST = 8.271806125530277e-25;  // 2^-80
+__device__ __forceinline__ bool sums_hold(const RmsNormBackward& p, const float2& s) {
+  return s.x >= p.least && s.x < 8.507059e37f && fabsf(s.y) < 8.507059e37f;  // 2^126; false of NaN
+}
+__device__ __forceinline__ float2 sums_of_four(const float4& h, const float4& dy, const float4& w) {
+  return make_float2(fmaf(h.x, h.x, h.y * h.y) + fmaf(h.z, h.z, h.w * h.w),
+                     fmaf(h.x, dy.x * w.x, h.y * (dy.y * w.y)) + fmaf(h.z, dy.z * w.z, h.w * (dy.w * w.w)));
+}
+__device__ __forceinline__ void add_exactly(double2& s, float h, float dy, float w) {
+  const double a = h;
+  s.x = fma(a, a, s.x);
+  s.y = fma(a, static_cast<double>(dy * w), s.y);
+}
+template <class T>
+__device__ __forceinline__ void sum_over_warp(T& s) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+    s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+  }
+}
+// The column of element j of a thread's four from `col` on, as load4 has them.
+template <int ACCESS>
+__device__ __forceinline__ int column_of(int col, int j) {
+  return ACCESS == ACCESS_LANES ? (col & ~127) + ((col & 127) >> 2) + 32 * j : col + j;
+}
+// What a row's gradient needs of its sums: r, and the mean of g n.
+__device__ __forceinline__ float2 backward_row(const RmsNormBackward& p, const double2& s) {
+  float unit;
+  const float r = inverse_root(fma(s.x, p.inv_cols, p.eps), &unit) * unit;
+  return make_float2(r, static_cast<float>(s.y * p.inv_cols * r));
+}
+__device__ __forceinline__ float4 normed(const float4& h, float r) { return make_float4(h.x * r, h.y * r, h.z * r, h.w * r); }
+// r (g - n mean(g n)) + dsum
+__device__ __forceinline__ float4 backward_of(const float4& n, const float4& dy, const float4& w, const float4& dsum, const float2& row) {
+  return make_float4(row.x * fmaf(-n.x, row.y, dy.x * w.x) + dsum.x, row.x * fmaf(-n.y, row.y, dy.y * w.y) + dsum.y,
+                     row.x * fmaf(-n.z, row.y, dy.z * w.z) + dsum.z, row.x * fmaf(-n.w, row.y, dy.w * w.w) + dsum.w);
+}
+__device__ __forceinline__ float4 added(const float4& part, const float4& dy, const float4& n) {
+  return make_float4(fmaf(dy.x, n.x, part.x), fmaf(dy.y, n.y, part.y), fmaf(dy.z, n.z, part.z), fmaf(dy.w, n.w, part.w));
+}
+// Rows of any length: h and dy are read twice, and the part of dweight is kept in the block's row of the workspace.  Four values are summed in
+// float32, the fours, of which a thread may have half a million, in 64 bits.
 template <int ACCESS>
 __global__ void __launch_bounds__(1024) rmsnorm_backward_kernel(const RmsNormBackward p) {
   constexpr int THREADS = 1024, PART = ACCESS == ACCESS_VECTOR ? ACCESS_SINGLE : ACCESS;  // the workspace starts on 4 bytes
-  __shared__ float2 shared[2][THREADS / 32];
+  __shared__ double2 shared[2][THREADS / 32];
   grid_launch_dependents();
   grid_dependency_wait();
   const int first = 4 * threadIdx.x;
-  const float inv_cols = 1.0f / static_cast<float>(p.cols), eps = static_cast<float>(p.eps);
   const long long padded = (p.cols + 127ll) / 128 * 128;
   float* const mine = p.workspace + static_cast<long long>(blockIdx.x) * p.cols;
   int turn = 0;
-  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const float *hr = p.h + row * p.ldh, *dyr = p.dy + row * p.lddy;
-    float2 s = make_float2(0.f, 0.f);  // of h^2 and of h * g
+    auto over_block = [&](double2 s) {
+      sum_over_warp(s);
+      if ((threadIdx.x & 31) == 0) shared[turn][threadIdx.x >> 5] = s;
+      __syncthreads();
+      s = shared[turn][threadIdx.x & 31];
+      sum_over_warp(s);
+      turn ^= 1;
+      return s;
+    };
+    double2 s = make_double2(0.0, 0.0);
     for (long long c = first; c < padded; c += 4 * THREADS) {
       const int col = static_cast<int>(c);
-      const float4 a = load4<ACCESS>(hr, col, p.cols), d = load4<ACCESS>(dyr, col, p.cols), w = load4<ACCESS>(p.weight, col, p.cols);
-      s.x += fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w);
-      s.y += fmaf(a.x, d.x * w.x, a.y * (d.y * w.y)) + fmaf(a.z, d.z * w.z, a.w * (d.w * w.w));
+      const float2 t = sums_of_four(load4<ACCESS>(hr, col, p.cols), load4<ACCESS>(dyr, col, p.cols), load4<ACCESS>(p.weight, col, p.cols));
+      s.x += t.x;
+      s.y += t.y;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
-      s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+    s = over_block(s);
+    if (!sums_hold(p, make_float2(static_cast<float>(s.x), static_cast<float>(s.y)))) {
+      s = make_double2(0.0, 0.0);
+      for (long long c = threadIdx.x; c < p.cols; c += THREADS) add_exactly(s, hr[c], dyr[c], p.weight[c]);
+      s = over_block(s);
     }
-    if ((threadIdx.x & 31) == 0) shared[turn][threadIdx.x >> 5] = s;
-    __syncthreads();
-    s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-      s.x += shared[turn][w].x;
-      s.y += shared[turn][w].y;
-    }
-    const float r = 1.0f / sqrtf(s.x * inv_cols + eps);
-    const float along = s.y * inv_cols * r * r;  // mean(g n) r: what h is multiplied by
+    const float2 of_row = backward_row(p, s);
     for (long long c = first; c < padded; c += 4 * THREADS) {
       const int col = static_cast<int>(c);
-      const float4 a = load4<ACCESS>(hr, col, p.cols), d = load4<ACCESS>(dyr, col, p.cols);
+      const float4 n = normed(load4<ACCESS>(hr, col, p.cols), of_row.x), d = load4<ACCESS>(dyr, col, p.cols);
       if (p.dweight) {
         float4 part = make_float4(0.f, 0.f, 0.f, 0.f);
         if (row != blockIdx.x) part = load4<PART>(mine, col, p.cols);
-        store4<PART>(mine, col, p.cols,
-                     make_float4(fmaf(d.x, a.x * r, part.x), fmaf(d.y, a.y * r, part.y), fmaf(d.z, a.z * r, part.z), fmaf(d.w, a.w * r, part.w)));
+        store4<PART>(mine, col, p.cols, added(part, d, n));
       }
       if (p.dx) {
-        const float4 w = load4<ACCESS>(p.weight, col, p.cols);
-        float4 o = make_float4(r * fmaf(-a.x, along, d.x * w.x), r * fmaf(-a.y, along, d.y * w.y), r * fmaf(-a.z, along, d.z * w.z),
-                               r * fmaf(-a.w, along, d.w * w.w));
-        if (p.dsum) {
-          const float4 t = load4<ACCESS>(p.dsum + row * p.ldds, col, p.cols);
-          o = make_float4(o.x + t.x, o.y + t.y, o.z + t.z, o.w + t.w);
-        }
-        store4<ACCESS>(p.dx + row * p.lddx, col, p.cols, o);
+        float4 ds = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p.dsum) ds = load4<ACCESS>(p.dsum + row * p.ldds, col, p.cols);
+        store4<ACCESS>(p.dx + row * p.lddx, col, p.cols, backward_of(n, d, load4<ACCESS>(p.weight, col, p.cols), ds, of_row));
       }
     }
   }
@@ -283,8 +333,9 @@ __global__ void __launch_bounds__(TG * G, 1) rmsnorm_backward_ring_kernel(const 
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[G * STAGES];
   __shared__ float2 sums[2][G * TG / 32];
+  __shared__ double2 exact_sums[G * TG / 32], exact_of_blocks[WIDE ? RMS_MAX_CLUSTER : 1];
   __shared__ float2 of_blocks[2][WIDE ? RMS_MAX_CLUSTER : 1];  // sums of the blocks of the cluster, rows in turn
-  __shared__ uint64_t sent[2];                                 // and the barriers that count them
+  __shared__ uint64_t sent[3];                                 // and the barriers that count them; the last: exact sums
   __shared__ int abort_word;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   const int group = threadIdx.x / TG, thread = threadIdx.x % TG, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = 4 * thread;
@@ -296,7 +347,8 @@ __global__ void __launch_bounds__(TG * G, 1) rmsnorm_backward_ring_kernel(const 
   uint8_t* mine = ring + group * STAGES * Ring::kStageBytes;
   if (threadIdx.x < G * STAGES) {
     mbar_init(smem_u32(&full[threadIdx.x]), 1);
-    if (WIDE && threadIdx.x < 2) mbar_init(smem_u32(&sent[threadIdx.x]), 1);
+    if (WIDE && threadIdx.x == 0)
+      for (int k = 0; k < 3; ++k) mbar_init(smem_u32(&sent[k]), 1);
     mbar_fence_init();
   }
   if (threadIdx.x == 0) abort_word = 0;
@@ -334,9 +386,15 @@ __global__ void __launch_bounds__(TG * G, 1) rmsnorm_backward_ring_kernel(const 
     part[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   int stage = 0, turn = 0;
-  uint32_t phase = 0, sent_phase = 0;
-  bool ok = true;
+  uint32_t phase = 0, sent_phase = 0, exact_phase = 0;
+  bool ok = true, ended = false;
+  // The next copies come behind the row's stores: in front of them they hold those up (8192 x 8191 199 us, 160 so).  Rows of a cluster that do not
+  // start on 16 bytes take them between their stores (4096 x 9999 139 -> 137, 1024 x 65535 189 -> 184; others lose: 6000 x 8196 141 -> 148).
+  constexpr bool kFetchWithin = WIDE && ACCESS == ACCESS_LANES;
   for (long long row = row0; row < p.rows; row += step) {
+    auto fetch_next = [&] {
+      if (thread == 0 && row + STAGES * step < p.rows) fetch(stage, row + STAGES * step);
+    };
     const uint8_t* from = mine + stage * Ring::kStageBytes;
     ok = mbar_wait_bounded(smem_u32(&full[group * STAGES + stage]), phase, &abort_word) && ok;
     float4 h[VECS], dy[VECS], ds[VECS];
@@ -357,36 +415,32 @@ __global__ void __launch_bounds__(TG * G, 1) rmsnorm_backward_ring_kernel(const 
         dy[v] = load4<ACCESS>(at + Ring::kArrayBytes / 4 + bulk_offset(dy0 + row * p.lddy), col, cols);
         if (p.dsum) ds[v] = load4<ACCESS>(at + 2 * (Ring::kArrayBytes / 4) + bulk_offset(dsum0 + row * p.ldds), col, cols);
       }
-      const float4 &a = h[v], &d = dy[v];
-      s.x += fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w);
-      s.y += fmaf(a.x, d.x * w[v].x, a.y * (d.y * w[v].y)) + fmaf(a.z, d.z * w[v].z, a.w * (d.w * w[v].w));
+      const float2 t = sums_of_four(h[v], dy[v], w[v]);
+      s.x += t.x;
+      s.y += t.y;
     }
-    auto over_warp = [](float2& x) {
-#pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        x.x += __shfl_xor_sync(0xffffffffu, x.x, o);
-        x.y += __shfl_xor_sync(0xffffffffu, x.y, o);
-      }
-    };
-    over_warp(s);
+    sum_over_warp(s);
     if (TG > 32) {
       if (lane == 0) sums[turn][warp] = s;
       ok = barrier_all(1 + group, TG, ok);  // the group has read the stage; all of it goes on, or none
     } else {
       ok = __all_sync(0xffffffffu, ok);
     }
-    if (!ok) break;
+    if (!ok) {
+      ended = true;
+      break;
+    }
     if constexpr (WIDE) {
       // A block sends its sums of the next row when all its threads have read those of this one, so that those of the row after that may be
-      // written over them.  Who gives up here does so at the next row, with its whole block.
+      // written over them; its exact sums come between two of these.  Who gives up does so at the block's next barrier, with the whole block.
       if (warp == 3) {
         s = lane < TG / 32 ? sums[turn][lane] : make_float2(0.f, 0.f);
-        over_warp(s);
+        sum_over_warp(s);
         const uint32_t bar = smem_u32(&sent[turn]);
         if (lane == 0) mbar_arrive_expect_tx(bar, blocks * 8);
-        if (lane < blocks) st_async_f32x2(map_to_cta(smem_u32(&of_blocks[turn][rank]), lane), s, map_to_cta(bar, lane));
+        if (lane < blocks) st_async_pair(map_to_cta(smem_u32(&of_blocks[turn][rank]), lane), s, map_to_cta(bar, lane));
       }
-      ok = mbar_wait_cluster(smem_u32(&sent[turn]), sent_phase, &abort_word);
+      ok = __all_sync(0xffffffffu, mbar_wait_cluster(smem_u32(&sent[turn]), sent_phase, &abort_word));
       s = make_float2(0.f, 0.f);
       for (int k = 0; k < blocks; ++k) {
         s.x += of_blocks[turn][k].x;
@@ -402,28 +456,81 @@ __global__ void __launch_bounds__(TG * G, 1) rmsnorm_backward_ring_kernel(const 
       }
     }
     turn ^= 1;
-    const float r = 1.0f / sqrtf(s.x * inv_cols + eps);
-    const float along = s.y * inv_cols * r * r;  // mean(g n) r: what h is multiplied by
+    bool hold = sums_hold(p, s) || (WIDE && !ok);
+    if (TG == 32) hold = __all_sync(0xffffffffu, hold);  // a branch of the whole warp: 16384 x 200 13.36 -> 13.16 us
+    if (hold) {
+      const float r = refined_root(s.x * inv_cols + eps);
+      const float2 of_row = make_float2(r, s.y * inv_cols * r);
 #pragma unroll
-    for (int v = 0; v < VECS; ++v) {
-      const float4 &a = h[v], &d = dy[v];
-      if (p.dx) {
-        const float4 o = make_float4(r * fmaf(-a.x, along, d.x * w[v].x) + ds[v].x, r * fmaf(-a.y, along, d.y * w[v].y) + ds[v].y,
-                                     r * fmaf(-a.z, along, d.z * w[v].z) + ds[v].z, r * fmaf(-a.w, along, d.w * w[v].w) + ds[v].w);
-        store4<ACCESS>(p.dx + col0 + row * p.lddx, first + v * 4 * TG, cols, o);
+      for (int v = 0; v < VECS; ++v) {
+        if (kFetchWithin && v == 1) fetch_next();
+        const float4 n = normed(h[v], of_row.x);
+        if (p.dx) store4<ACCESS>(p.dx + col0 + row * p.lddx, first + v * 4 * TG, cols, backward_of(n, dy[v], w[v], ds[v], of_row));
+        part[v] = added(part[v], dy[v], n);
       }
-      part[v].x = fmaf(d.x, a.x * r, part[v].x);
-      part[v].y = fmaf(d.y, a.y * r, part[v].y);
-      part[v].z = fmaf(d.z, a.z * r, part[v].z);
-      part[v].w = fmaf(d.w, a.w * r, part[v].w);
+    } else {
+      // All of the group, which has the same sums, does them over.  A warp that gave up is not here but at the next row's barrier, or behind the
+      // loop: there it brings its false, and all of them end.  Small loops over the row as it lies in global memory: held in registers
+      // throughout it made the kernel spill (8192 x 8191 160 -> 173 us).
+      double2 exact = make_double2(0.0, 0.0);
+#pragma unroll 1
+      for (int k = 0; k < 4 * VECS; ++k) {
+        const int col = column_of<ACCESS>(first + (k >> 2) * 4 * TG, k & 3);
+        if (col >= cols) continue;
+        add_exactly(exact, h0[row * p.ldh + col], dy0[row * p.lddy + col], weight[col]);
+      }
+      sum_over_warp(exact);
+      if (TG > 32) {
+        if (lane == 0) exact_sums[warp] = exact;
+        ok = barrier_all(1 + group, TG, ok);
+        if (!ok) {
+          ended = true;
+          break;
+        }
+        exact = make_double2(0.0, 0.0);
+        if constexpr (WIDE) {
+          if (warp == 3) {
+            if (lane < TG / 32) exact = exact_sums[lane];
+            sum_over_warp(exact);
+            const uint32_t bar = smem_u32(&sent[2]);
+            if (lane == 0) mbar_arrive_expect_tx(bar, blocks * 16);
+            if (lane < blocks) st_async_pair(map_to_cta(smem_u32(&exact_of_blocks[rank]), lane), exact, map_to_cta(bar, lane));
+            exact = make_double2(0.0, 0.0);
+          }
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(smem_u32(&sent[2]), exact_phase, &abort_word));
+          exact_phase ^= 1u;
+        }
+        const double2* const parts = WIDE ? exact_of_blocks : exact_sums + group * (TG / 32);
+        const int count = WIDE ? blocks : TG / 32;
+#pragma unroll 1
+        for (int k = 0; k < count; ++k) {
+          exact.x += parts[k].x;
+          exact.y += parts[k].y;
+        }
+      }
+      const float2 of_row = backward_row(p, exact);
+#pragma unroll 1
+      for (int k = 0; k < 4 * VECS; ++k) {
+        const int col = column_of<ACCESS>(first + (k >> 2) * 4 * TG, k & 3);
+        if (col >= cols) continue;
+        const float n = h0[row * p.ldh + col] * of_row.x, d = dy0[row * p.lddy + col];
+#pragma unroll
+        for (int u = 0; u < VECS; ++u) {
+          if (k == 4 * u) part[u].x = fmaf(d, n, part[u].x);
+          if (k == 4 * u + 1) part[u].y = fmaf(d, n, part[u].y);
+          if (k == 4 * u + 2) part[u].z = fmaf(d, n, part[u].z);
+          if (k == 4 * u + 3) part[u].w = fmaf(d, n, part[u].w);
+        }
+        if (p.dx) p.dx[col0 + row * p.lddx + col] = of_row.x * fmaf(-n, of_row.y, d * weight[col]) + (p.dsum ? dsum0[row * p.ldds + col] : 0.0f);
+      }
     }
-    // behind the row's stores: in front of them the copies hold those up (8192 x 8191 199 us, 160 so)
-    if (thread == 0 && row + STAGES * step < p.rows) fetch(stage, row + STAGES * step);
+    if (!kFetchWithin || !hold) fetch_next();
     if (++stage == STAGES) {
       stage = 0;
       phase ^= 1u;
     }
   }
+  if (WIDE && !ended) ok = barrier_all(1, TG, ok);
   if (!ok) {
     atomicCAS(p.status, 0, 0x3100 | group);
     wait_for_copies();

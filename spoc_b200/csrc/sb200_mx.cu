@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <limits.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <algorithm>
@@ -544,6 +545,8 @@ int sb200_rmsnorm_backward_f32(int dev, uint64_t stream, int64_t rows, int64_t c
   p.lddx = lddx;
   p.rows = rows;
   p.cols = static_cast<int>(cols);
+  p.least = eps < RMS_LEAST ? static_cast<float>(RMS_LEAST) : eps < 1e38 ? 0.0f : INFINITY;  // an eps past float32: no row's sums hold
+  p.inv_cols = 1.0 / static_cast<double>(cols);
   p.eps = eps;
   const bool vec = cols % 4 == 0 && on_16(sum, lds) && on_16(weight, 0) && on_16(dy, lddy) && (!dsum || on_16(dsum, ldds)) && (!dx || on_16(dx, lddx));
   p.status = d.status;

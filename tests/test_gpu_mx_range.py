@@ -1,0 +1,55 @@
+"""The norm and its gradient from float32's smallest values to its largest, against 64 bits."""
+import numpy as np
+import pytest
+
+from tests import mx_ref as R
+from tests.test_gpu_mx import keep, run_backward  # noqa: F401  (a fixture)
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24      # half a step of float32
+
+
+def check_gradient(got, h, w, dy, dsum, eps):
+    """In units of U.  A float32 sum adds a value in 28 roundings at most (three within four values, four fours, five steps over a warp, sixteen warps), so
+    that r is off by 14, 2 of the mean's own and 3 of the root: 19; n = h r by 20, g = dy w by 1, mean(g n) by 28 + 1 + 19 and three products, 51
+    of mean(|g n|); r (g - n mean(g n)) by 1 + 1 + 20 of |g| and 71 + 2 + 20 of |n mean|, the addition of dsum by one more: 94.  Results below 2^-126
+    are off by half of 2^-149 for each of the last two besides.  dweight adds a row at a time; the zeros of blocks without a row add exactly."""
+    dx, dw = R.rmsnorm_backward(h, w, dy, dsum, eps)
+    h, w, dy = (v.astype(np.float64) for v in (h, w, dy))
+    r = 1 / np.sqrt((h * h).mean(-1, keepdims=True) + eps)
+    n, g = np.abs(h * r), np.abs(dy * w)
+    size = r * (g + n * (g * n).mean(-1, keepdims=True)) + (0 if dsum is None else np.abs(dsum))
+    assert np.all(np.abs(got[0] - dx) <= 94 * U * size + 2.0 ** -149)
+    assert np.all(np.abs(got[1] - dw) <= (h.shape[0] + 21) * U * (np.abs(dy) * n).sum(0))
+
+
+# every width of a warp's, a block's and a cluster's row, and rows read twice
+@pytest.mark.parametrize("cols", [1, 33, 128, 250, 400, 512, 1000, 2048, 4096, 4099, 8192, 9000, 20004, 65536, 65540, 70001])
+def test_gradient_of_rows_from_the_smallest_to_the_largest(keep, device, cols):  # noqa: F811
+    """Rows of 1e-37 to 1e37, whose squares lie up to 2^37 times past either end of float32, side by side."""
+    rng = np.random.default_rng(cols)
+    scale = np.array([1e-37, 1e-30, 1e-24, 1e-19, 1e-18, 1.0, 6e16, 3e17, 1e18, 1e19, 1e25, 1e31, 5e36])[:, None]
+    rows = scale.size
+    h = (rng.choice([-1.0, 1.0], (rows, cols)) * rng.uniform(1.0, 1.8, (rows, cols)) * scale).astype(np.float32)
+    w, dy = rng.normal(size=cols).astype(np.float32), rng.normal(size=(rows, cols)).astype(np.float32)
+    dsum = (rng.normal(size=(rows, cols)) / scale).astype(np.float32) if cols % 2 else None
+    pad, offset, in_place = [(0, 0, "sum"), (3, 1, None), (4, 0, "dy")][cols % 3]
+    check_gradient(run_backward(keep, device, h, w, dy, dsum, 0.0, pad, offset, in_place), h, w, dy, dsum, 0.0)
+
+
+@pytest.mark.parametrize("eps", [1e-70, 1e-40, 1e-20, 1e30])
+@pytest.mark.parametrize("cols", [100, 3000, 9001, 66000])
+def test_gradient_of_zeros_and_small_rows_beside_eps(keep, device, cols, eps):  # noqa: F811
+    """Where the squares vanish beside eps, n does and r is 1 / sqrt(eps)."""
+    rng = np.random.default_rng(cols)
+    h = (rng.normal(size=(6, cols)) * np.array([0.0, 1e-44, 1e-37, 1e-30, 1.0, 1e20])[:, None]).astype(np.float32)
+    w, dy = rng.normal(size=cols).astype(np.float32), rng.normal(size=(6, cols)).astype(np.float32)
+    check_gradient(run_backward(keep, device, h, w, dy, None, eps), h, w, dy, None, eps)
+
+
+def test_gradient_of_large_gradients(keep, device):  # noqa: F811
+    """Products of h and g past float32, whose mean is an ordinary number of g's size."""
+    rng = np.random.default_rng(3)
+    h = (rng.normal(size=(7, 700)) * 1e25).astype(np.float32)
+    w, dy = rng.normal(size=700).astype(np.float32), (rng.normal(size=(7, 700)) * 1e20).astype(np.float32)
+    check_gradient(run_backward(keep, device, h, w, dy, None, 1e-5), h, w, dy, None, 1e-5)
