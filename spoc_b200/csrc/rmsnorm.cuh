@@ -73,7 +73,10 @@ __device__ __forceinline__ float refined_root(float m) {
 __device__ __forceinline__ float inverse_root(double mean, float* unit) {
   const int half = (static_cast<int>(__double2hiint(mean) >> 20 & 0x7ff) - 1023) / 2;
   const float u = abs(half) < 45 ? 1.0f : __uint_as_float(static_cast<uint32_t>(min(max(127 - half, 1), 254)) << 23);
-  const float m = static_cast<float>(mean * u * u), s = refined_root(m);
+  float m = static_cast<float>(mean * u * u);
+  // Only the eps of a row of zeros is so small: one of float32's smallest values in 2^31 makes a mean of 2^-329, and m 2^-75.
+  if (m < 1.17549435e-38f && mean > 0.0) m = 1.17549435e-38f;
+  const float s = refined_root(m);
   *unit = u;
   return m < INFINITY ? s : rsqrtf(m);  // of an infinite mean 0
 }

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from tests import mx_ref as R
-from tests.test_gpu_mx import keep, run_backward  # noqa: F401  (a fixture)
+from tests.test_gpu_mx import keep, run_backward, run_norm  # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24      # half a step of float32
@@ -53,3 +53,20 @@ def test_gradient_of_large_gradients(keep, device):  # noqa: F811
     h = (rng.normal(size=(7, 700)) * 1e25).astype(np.float32)
     w, dy = rng.normal(size=700).astype(np.float32), (rng.normal(size=(7, 700)) * 1e20).astype(np.float32)
     check_gradient(run_backward(keep, device, h, w, dy, None, 1e-5), h, w, dy, None, 1e-5)
+
+
+@pytest.mark.parametrize("fmt", [0, R.FP8, R.FP4])
+@pytest.mark.parametrize("eps", [5e-324, 1e-300, 1e-140, 1e-120, 1e-100, 1e-30, 1e300, float("inf")])
+@pytest.mark.parametrize("cols", [100, 1500, 33000])
+def test_norm_of_zeros_beside_any_eps(keep, device, cols, eps, fmt):  # noqa: F811
+    """A row of zeros has the norm zero wherever eps is not; rows beside it are what they are.  2^-22: the scale is off by two units of U, two products by one each."""
+    rng = np.random.default_rng(cols)
+    x = (rng.normal(size=(5, cols)) * np.array([0.0, 1.0, 0.0, 1e-44, 1e30])[:, None]).astype(np.float32)
+    w = rng.normal(size=cols).astype(np.float32)
+    _, y, q = run_norm(keep, device, x, None, w, eps, fmt, 1)
+    want = R.rmsnorm(x, None, w, eps)[1]
+    assert np.all(np.abs(y - want) <= 2.0 ** -22 * np.abs(want) + 2.0 ** -148 * np.maximum(1, np.abs(w)))
+    assert np.all(y[[0, 2]] == 0)
+    if fmt:
+        codes, scales = R.quantize(want, fmt)
+        assert np.array_equal(q[1], scales) and np.array_equal(q[0], codes)
