@@ -201,7 +201,7 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         for (int it = 0; it < k_blocks; ++it) {
           const int kb = k0 + it;
           if (!mbar_wait_bounded(smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) {
-            atomicCAS(p.status, 0, 0x2100 | (rank << 4) | stage);
+            atomicCAS(p.status, 0, 0x4100 | (rank << 4) | stage);
             ok = false;
             break;
           }
@@ -258,7 +258,7 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         if (n_tiles >= behind) {
           const uint32_t free = smem_u32(&tmem_empty_bar[(n_tiles - behind) & 1]), phase_of = ((n_tiles - behind) >> 1) & 1;
           if (!(CTAS == 2 ? mbar_wait_cluster(free, phase_of, abort_flag) : mbar_wait_bounded(free, phase_of, abort_flag))) {
-            atomicCAS(p.status, 0, 0x2200 | acc);
+            atomicCAS(p.status, 0, 0x4200 | acc);
             ok = false;
             break;
           }
@@ -275,7 +275,7 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             }
           }
           if (!ready) {
-            atomicCAS(p.status, 0, 0x2300 | stage);
+            atomicCAS(p.status, 0, 0x4300 | stage);
             ok = false;
             break;
           }
@@ -354,7 +354,7 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       }
       const bool landed = mbar_wait_bounded(smem_u32(&tmem_full_bar[acc]), acc_phase, abort_flag);
       if (!__all_sync(0xffffffffu, landed)) {
-        if (lane == 0) atomicCAS(p.status, 0, 0x2400 | (rank << 4) | acc);
+        if (lane == 0) atomicCAS(p.status, 0, 0x4400 | (rank << 4) | acc);
         ok = false;
         break;
       }

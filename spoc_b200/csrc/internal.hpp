@@ -17,6 +17,19 @@ int set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3
 // A failed CUDA call, as a status.
 int set_cuda_error(cudaError_t e, const char* what);
 
+// The kernel that a wait's number in the status word is from: the numbers of each begin with a digit of its own.
+inline const char* waiting_kernel(int site) {
+  switch (site >> 12) {
+    case 0: return "wait_timeout_probe_kernel";
+    case 1: return "gemm_pair_kernel";
+    case 2: return "gemm_convert_kernel";
+    case 3: return "gemm_split_kernel";
+    case 4: return "gemm_mx_kernel";
+    case 5: return "rmsnorm_backward_ring_kernel";
+    default: return "a kernel";
+  }
+}
+
 // What an operator outside sb200_shim.cu needs of a device.
 struct OperatorDevice {
   int index, sm_count;

@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(TG * G, 1) rmsnorm_backward_ring_kernel(const 
   }
   if (WIDE && !ended) ok = barrier_all(1, TG, ok);
   if (!ok) {
-    atomicCAS(p.status, 0, 0x3100 | group);
+    atomicCAS(p.status, 0, 0x5100 | group);
     wait_for_copies();
   }
   if (WIDE) {  // no block retires while another can still send to it

@@ -165,7 +165,7 @@ int check_status_word(DeviceState& d, bool device_wide = false) {
   CU_TRY(cudaMemcpy(&h, d.status, sizeof(int), cudaMemcpyDeviceToHost));
   if (h != 0) {
     cudaMemset(d.status, 0, sizeof(int));
-    return fail(SB200_ERR_TIMEOUT, "a bounded device-side wait expired in the GEMM pipeline (site 0x%x)", h);
+    return fail(SB200_ERR_TIMEOUT, "a bounded device-side wait expired in %s (site 0x%x)", waiting_kernel(h), h);
   }
   return SB200_OK;
 }
@@ -3236,7 +3236,7 @@ extern "C" int sb200_gemm_f32_noalloc(int dev, uint64_t stream, int mode, int64_
   CU_TRY(cudaMemcpy(&flag, nd->status, sizeof(int), cudaMemcpyDeviceToHost));
   if (flag != 0) {
     CU_TRY(cudaMemset(nd->status, 0, sizeof(int)));
-    return fail(SB200_ERR_TIMEOUT, "a bounded device-side wait expired in the GEMM pipeline (site 0x%x)", flag);
+    return fail(SB200_ERR_TIMEOUT, "a bounded device-side wait expired in %s (site 0x%x)", waiting_kernel(flag), flag);
   }
   return SB200_OK;
 }
