@@ -11,6 +11,7 @@
 
 #include "../../include/sb200.h"
 #include "gemm_mx.cuh"
+#include "gemm_mx_plan.hpp"
 #include "internal.hpp"
 #include "microscale.cuh"
 #include "rmsnorm.cuh"
@@ -169,45 +170,6 @@ int launch_rmsnorm_backward(const OperatorDevice& d, cudaStream_t st, const RmsN
 }
 
 // --------------------------------------------------------------- product
-// Tiles: 128 (256: pairs) columns of D by bt rows.
-struct MxShape {
-  int ctas = 1, bt = 128, splits = 1;
-};
-int64_t mx_tiles(const MxShape& s, int64_t M, int64_t N) { return (N + 128 * s.ctas - 1) / (128 * s.ctas) * ((M + s.bt - 1) / s.bt); }
-
-// The shape with the least estimated time.  Measured on one B200, operands from L2 and HBM, in us: a launch with one k-block 3.3; a k-block 0.165 and
-// 0.4 ns a row of A in a block's tile (4 loads, 4 MMAs and a round of barriers, whatever the width up to 64 rows), half as much again where all
-// SMs load at once (128 x 2048 x 16384 0.21, 2048 x 4096 x 4096 0.29); in pairs 0.22 to 0.28 for 128 rows and 0.31 to 0.42 for 256; the last
-// epilogue 6 ns a row; a k-loop divided within a cluster 1.1 and 30 ns for every row a block sends (1 x 4096 x 4096 8.6 -> 5.7 us in four,
-// 64 x 4096 x 4096 9.3 -> 7.3).
-MxShape choose_mx_shape(int64_t M, int64_t N, int64_t k_blocks, int sm_count) {
-  MxShape best;
-  double best_us = 0.0;
-  auto consider = [&](int ctas, int bt, int splits) {
-    MxShape s;
-    s.ctas = ctas;
-    s.bt = bt;
-    s.splits = splits;
-    const int64_t tiles = mx_tiles(s, M, N), units = std::max(1, sm_count / ctas);
-    if (splits > 1 && tiles > cluster_capacity(splits, sm_count)) return;  // all clusters at once
-    const int64_t per_item = (k_blocks + splits - 1) / splits, waves = splits > 1 ? 1 : (tiles + units - 1) / units;
-    const double busy = std::min(1.0, static_cast<double>(tiles) * splits / units);
-    const double k_block = ctas == 1 ? (0.165 + 0.0004 * bt) * (bt == 128 ? 1.0 + 0.4 * busy : 1.0) : bt == 256 ? 0.31 + 0.11 * busy : 0.19 + 0.0003 * bt + 0.06 * busy;
-    double us = 3.3 + static_cast<double>(waves * per_item) * k_block + 0.006 * bt + 0.5 * static_cast<double>(waves - 1);
-    if (splits > 1) us += 1.1 + 0.03 * bt * (splits - 1) / splits;
-    if (best_us == 0.0 || us < 0.97 * best_us) {
-      best = s;
-      best_us = us;
-    }
-  };
-  const int narrow = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  for (int splits = 1; splits <= MXG_MAX_SPLITS; ++splits)
-    if (k_blocks >= 2 * splits || splits == 1) consider(1, narrow, splits);
-  if (narrow >= 64) consider(2, narrow, 1);
-  if (M > 128) consider(2, 256, 1);
-  return best;
-}
-
 template <bool FP4, int CTAS, int GROUPS, bool IN_CLUSTER = false>
 int launch_mx(const OperatorDevice& d, cudaStream_t st, const CUtensorMap (&maps)[6], const MxGemm& p) {
   auto kernel = gemm_mx_kernel<FP4, CTAS, GROUPS, IN_CLUSTER>;
@@ -231,37 +193,20 @@ int launch_mx(const OperatorDevice& d, cudaStream_t st, const CUtensorMap (&maps
 int run_gemm_mx(const OperatorDevice& d, cudaStream_t st, int format_a, int format_b, int64_t K, uint64_t a_codes, uint64_t a_scales, uint64_t b_codes,
                 uint64_t b_scales, MxGemm p) {
   const bool fp4 = format_a == SB200_MX_FP4 && format_b == SB200_MX_FP4;
-  p.chunks = static_cast<int>(chunks_of(K));
-  p.num_k_blocks = fp4 ? (p.chunks + 1) / 2 : p.chunks;
-  const MxShape s = choose_mx_shape(p.M, p.N, p.num_k_blocks, d.sm_count);
-  const int64_t tiles = mx_tiles(s, p.M, p.N);
-  if (tiles > INT_MAX / 16) return set_error(SB200_ERR_TOO_LARGE, "gemm_mx: %lld tiles", (long long)tiles);
+  const MxPlan s = plan_gemm_mx(fp4, p.M, p.N, K, d.sm_count);
+  if (s.tiles > INT_MAX / 16) return set_error(SB200_ERR_TOO_LARGE, "gemm_mx: %lld tiles", (long long)s.tiles);
+  p.chunks = s.chunks;
+  p.num_k_blocks = s.num_k_blocks;
   p.bt = s.bt;
   p.tiles_f = static_cast<int>((p.N + 128ll * s.ctas - 1) / (128 * s.ctas));
   p.tiles_t = static_cast<int>((p.M + static_cast<int64_t>(s.bt) - 1) / s.bt);
-  const int groups = s.bt > 128 ? 2 : 1;  // tiles of 128 rows of A's scales that a tile touches
-  p.split_k_blocks = (p.num_k_blocks + s.splits - 1) / s.splits;
-  p.splits = (p.num_k_blocks + p.split_k_blocks - 1) / p.split_k_blocks;  // the last one has something to do
-  const int scale_tiles = fp4 ? 2 : 1;
-  const int x_bytes = s.bt / s.ctas * 128, sf_bytes = scale_tiles * MX_TILE_BYTES * (1 + groups);
-  p.stage_bytes = (static_cast<int>(MXG_W_BYTES) + x_bytes + sf_bytes + 1023) / 1024 * 1024;
-  p.stages = std::min(MXG_MAX_STAGES, MXG_RING_BYTES / p.stage_bytes);
-  const int sf_cols = 4 * scale_tiles * (1 + groups), units = d.sm_count / s.ctas;
-  if (tiles <= units || p.splits > 1) {
-    // A tile a block: no more stages than k-blocks, one accumulator, and no more tensor memory than that takes, so that the blocks of the
-    // launch behind this one can set themselves up beside these.
-    p.stages = std::max(1, std::min(p.stages, p.split_k_blocks));
-    const int held = std::max(32, s.bt);
-    p.slots = std::min(p.stages, (MXG_TMEM_COLS - held) / sf_cols);
-    p.tmem_cols = 32;
-    while (p.tmem_cols < held + p.slots * sf_cols) p.tmem_cols *= 2;
-    p.acc1 = s.bt;
-  } else {
-    // two accumulators, which overlap by 64 columns at most
-    p.slots = std::min(p.stages, (MXG_TMEM_COLS - 2 * s.bt + (s.bt == 256 ? 64 : 0)) / sf_cols);
-    p.tmem_cols = MXG_TMEM_COLS;
-    p.acc1 = std::min(256, MXG_TMEM_COLS - p.slots * sf_cols - s.bt);
-  }
+  p.splits = s.splits;
+  p.split_k_blocks = s.split_k_blocks;
+  p.stages = s.stages;
+  p.stage_bytes = s.stage_bytes;
+  p.slots = s.slots;
+  p.tmem_cols = s.tmem_cols;
+  p.acc1 = s.acc1;
   // spread: 4-bit codes that TMA spreads to a byte a value; a barrier counts the bytes that it reads
   const bool spread_w = !fp4 && format_b == SB200_MX_FP4, spread_x = !fp4 && format_a == SB200_MX_FP4;
   p.w_row_bytes = spread_w ? 64 : 128;
@@ -279,7 +224,7 @@ int run_gemm_mx(const OperatorDevice& d, cudaStream_t st, int format_a, int form
   auto scales_map = [&](CUtensorMap* map, uint64_t scales, int64_t rows) {
     return encode_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, as_ptr<void>(scales), MX_TILE_BYTES / 4,
                                 static_cast<uint64_t>((rows + 127) / 128) * p.chunks, MX_TILE_BYTES, MX_TILE_BYTES / 4,
-                                static_cast<uint32_t>(scale_tiles), CU_TENSOR_MAP_SWIZZLE_NONE);
+                                fp4 ? 2 : 1, CU_TENSOR_MAP_SWIZZLE_NONE);
   };
   const int part_t = s.bt / s.ctas;
   const int w_tail = p.N % 128 ? p.N % 128 : 128, x_tail = p.M % part_t ? p.M % part_t : part_t;
@@ -295,7 +240,7 @@ int run_gemm_mx(const OperatorDevice& d, cudaStream_t st, int format_a, int form
   if (x_tail == part_t) maps[3] = maps[1];
   if (p.splits > 1) return fp4 ? launch_mx<true, 1, 1, true>(d, st, maps, p) : launch_mx<false, 1, 1, true>(d, st, maps, p);
   if (s.ctas == 1) return fp4 ? launch_mx<true, 1, 1>(d, st, maps, p) : launch_mx<false, 1, 1>(d, st, maps, p);
-  if (groups == 1) return fp4 ? launch_mx<true, 2, 1>(d, st, maps, p) : launch_mx<false, 2, 1>(d, st, maps, p);
+  if (s.groups == 1) return fp4 ? launch_mx<true, 2, 1>(d, st, maps, p) : launch_mx<false, 2, 1>(d, st, maps, p);
   return fp4 ? launch_mx<true, 2, 2>(d, st, maps, p) : launch_mx<false, 2, 2>(d, st, maps, p);
 }
 
