@@ -1,4 +1,5 @@
-"""How products of microscaled matrices are run, on the host: plans within the chip's limits, and no candidate that is never taken."""
+"""How products of microscaled matrices are run, on the host: plans within the chip's limits, no candidate that is never taken, and GPU tests that take
+every form."""
 import os
 import random
 import subprocess
@@ -6,6 +7,8 @@ import subprocess
 import pytest
 
 from spoc_b200.build import CSRC, _nvcc
+from tests.test_gpu_mx import SHAPES
+from tests.test_gpu_mx_forms import FORMS
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SMS = 148
@@ -58,3 +61,37 @@ def test_every_candidate_is_taken_by_some_size(plans):
         considered |= {(ctas, bt, splits > 1) for ctas, bt, splits in candidates}
         taken.add((p["ctas"], p["bt"], p["splits"] > 1))
     assert taken == considered
+
+
+def test_the_gpu_tests_take_every_form(plans):
+    sizes = [(fp4, *s) for s in SHAPES + FORMS for fp4 in (0, 1)]
+    seen = set()
+    for (fp4, m, n, k), p, _ in plans(sizes):
+        units = SMS // p["ctas"]
+        how = "divided" if p["splits"] > 1 else "several" if p["tiles"] > units else "one"
+        form = (fp4, p["ctas"], p["bt"], how)
+        seen |= {form}
+        if p["split_k_blocks"] > p["stages"]:
+            seen.add(form[:3] + ("ring turns",))
+        if how == "several" and p["tiles"] > 2 * units:
+            seen.add((fp4, p["ctas"], "accumulators come round"))
+        if p["slots"] < p["stages"]:
+            seen.add((fp4, "fewer slots than stages"))
+        if how == "several" and p["acc1"] < p["bt"]:
+            seen.add((fp4, "accumulators overlap"))
+        if p["ctas"] == 2:
+            if 0 < n % 256 <= 128:
+                seen.add((fp4, p["bt"], "a pair's second block past the last column"))
+            if 0 < m % p["bt"] <= p["bt"] // 2:
+                seen.add((fp4, p["bt"], "a pair's second block past the last row"))
+        if fp4 and p["chunks"] % 2:
+            seen.add((p["ctas"], p["bt"], "half a k-block"))
+    want = set()
+    for fp4 in (0, 1):
+        want |= {(fp4, 1, bt, how) for bt in (16, 32, 64, 128) for how in ("one", "divided", "several")}
+        want |= {(fp4, 2, bt, how) for bt in (128, 256) for how in ("one", "several", "ring turns")}
+        want |= {(fp4, 1, 16, "ring turns"), (fp4, 1, 128, "ring turns"), (fp4, 1, "accumulators come round"), (fp4, 2, "accumulators come round")}
+        want |= {(fp4, "fewer slots than stages"), (fp4, "accumulators overlap")}
+        want |= {(fp4, bt, f"a pair's second block past the last {what}") for bt in (128, 256) for what in ("column", "row")}
+    want |= {(1, bt, "half a k-block") for bt in (16, 64, 128)} | {(2, bt, "half a k-block") for bt in (128, 256)}
+    assert want <= seen, sorted(map(str, want - seen))
