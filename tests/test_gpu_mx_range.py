@@ -9,18 +9,19 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24      # half a step of float32
 
 
-def check_gradient(got, h, w, dy, dsum, eps):
+def check_gradient(got, h, w, dy, dsum, eps, additions=None):
     """In units of U.  A float32 sum adds a value in 28 roundings at most (three within four values, four fours, five steps over a warp, sixteen warps), so
     that r is off by 14, 2 of the mean's own and 3 of the root: 19; n = h r by 20, g = dy w by 1, mean(g n) by 28 + 1 + 19 and three products, 51
     of mean(|g n|); r (g - n mean(g n)) by 1 + 1 + 20 of |g| and 71 + 2 + 20 of |n mean|, the addition of dsum by one more: 94.  Results below 2^-126
-    are off by half of 2^-149 for each of the last two besides.  dweight adds a row at a time; the zeros of blocks without a row add exactly."""
+    are off by half of 2^-149 for each of the last two besides.  dweight adds a row at a time, or as few as `additions` says; the
+    zeros of blocks without a row add exactly."""
     dx, dw = R.rmsnorm_backward(h, w, dy, dsum, eps)
     h, w, dy = (v.astype(np.float64) for v in (h, w, dy))
     r = 1 / np.sqrt((h * h).mean(-1, keepdims=True) + eps)
     n, g = np.abs(h * r), np.abs(dy * w)
     size = r * (g + n * (g * n).mean(-1, keepdims=True)) + (0 if dsum is None else np.abs(dsum))
     assert np.all(np.abs(got[0] - dx) <= 94 * U * size + 2.0 ** -149)
-    assert np.all(np.abs(got[1] - dw) <= (h.shape[0] + 21) * U * (np.abs(dy) * n).sum(0))
+    assert np.all(np.abs(got[1] - dw) <= ((additions or h.shape[0]) + 21) * U * (np.abs(dy) * n).sum(0))
 
 
 # every width of a warp's, a block's and a cluster's row, and rows read twice
