@@ -57,10 +57,17 @@ __device__ __forceinline__ float round_to_odd(double y) {
 }
 
 template <bool FP4>
-__device__ __noinline__ void rmsnorm_chunk_exact(float4 h, float4 w, double mean, uint8_t* codes, uint8_t* scales, int lane) {
+__device__ __noinline__ void rmsnorm_chunk_exact(float4 h, float4 w, double mean, uint8_t* codes, uint8_t* scales, int col, int cols) {
+  const int lane = threadIdx.x & 31, left = cols - col;
   const double scale = 1.0 / sqrt(mean);
-  const float4 y = make_float4(round_to_odd(h.x * scale * w.x), round_to_odd(h.y * scale * w.y), round_to_odd(h.z * scale * w.z),
-                               round_to_odd(h.w * scale * w.w));
+  float4 y = make_float4(round_to_odd(h.x * scale * w.x), round_to_odd(h.y * scale * w.y), round_to_odd(h.z * scale * w.z),
+                         round_to_odd(h.w * scale * w.w));
+  if (left < 4) {  // past K are zeros, where the mean is no number too
+    if (left < 1) y.x = 0.f;
+    if (left < 2) y.y = 0.f;
+    if (left < 3) y.z = 0.f;
+    y.w = 0.f;
+  }
   mx_store_chunk<FP4>(y, mx_scale_of<FP4>(largest_of_block(y)), codes, scales, lane);
 }
 
@@ -124,7 +131,7 @@ __device__ __forceinline__ void rmsnorm_emit(const RmsNorm& p, const RmsRow& row
     if (__any_sync(0xffffffffu, again)) {
       if (m == 0 && low == high) again = (abs_bits(h.x) | abs_bits(h.y) | abs_bits(h.z) | abs_bits(h.w)) != 0;
       if (__any_sync(0xffffffffu, again)) {
-        rmsnorm_chunk_exact<FP4>(h, w, row.mean, codes, scales, lane);
+        rmsnorm_chunk_exact<FP4>(h, w, row.mean, codes, scales, col, p.cols);
         return;
       }
     }

@@ -71,3 +71,21 @@ def test_norm_of_zeros_beside_any_eps(keep, device, cols, eps, fmt):  # noqa: F8
     if fmt:
         codes, scales = R.quantize(want, fmt)
         assert np.array_equal(q[1], scales) and np.array_equal(q[0], codes)
+
+
+@pytest.mark.parametrize("fmt", R.FORMATS)
+@pytest.mark.parametrize("cols", [1, 32, 33, 100, 130, 600, 1057, 2100, 4097, 33000])
+def test_rows_that_are_not_numbers_leave_what_is_past_them_zero(keep, device, cols, fmt):  # noqa: F811
+    """Codes and scales past K are zeros whatever the row: NaN, infinite, or zero beside an eps of zero."""
+    rng = np.random.default_rng(cols)
+    x, w = rng.normal(size=(5, cols)).astype(np.float32), rng.normal(size=cols).astype(np.float32)
+    x[0, 0], x[1, cols // 2], x[2] = np.nan, np.inf, 0.0
+    _, _, (codes, scales) = run_norm(keep, device, x, None, w, 0.0, fmt)
+    with np.errstate(invalid="ignore"):
+        want_codes, want_scales = R.quantize(R.rmsnorm(x, None, w, 0.0)[1], fmt)
+    assert np.array_equal(scales, want_scales)
+    assert np.array_equal(codes[3:], want_codes[3:])
+    per_byte = 2 if fmt == R.FP4 else 1
+    assert not codes[:, -(-cols // per_byte):].any()
+    if cols % per_byte:
+        assert not (codes[:, cols // per_byte] >> 4).any()
