@@ -418,9 +418,10 @@ SB200_API int sb200_chain_triad_square_f32(int dev, uint64_t stream, uint64_t d,
  *           (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4 of tile (r / 128) * ceil(K / 128) + b / 4.  Zero past the last row and K.
  * Both start on 32 bytes (SB200_ERR_ALIGNMENT).  The scale of a block is 2^max(floor(log2 m) - e, -127), m the largest magnitude in it, e = 8
  * for e4m3 and 2 for e2m1; values are rounded to the nearest, ties to even, and held at the type's largest (448, 6).  A block with a
- * NaN or an infinity gets the scale NaN.  As with the other direct operators, calls may be issued on any streams, buffers of this
- * library are checked for their extent, and a call enqueues nothing but kernel launches; these use no scratch of the library's, so that
- * calls on several streams run side by side and graphs of them may be replayed side by side. */
+ * NaN or an infinity gets the scale NaN, and what a product sums with it is NaN; SB200_ACT_RELU makes 0 of that, as in sb200_gemm_f32.
+ * As with the other direct operators, calls may be issued on any streams, buffers of this library are checked for their extent, and a call
+ * enqueues nothing but kernel launches; these use no scratch of the library's, so that calls on several streams run side by side and graphs of
+ * them may be replayed side by side. */
 #define SB200_MX_FP8 8
 #define SB200_MX_FP4 4
 /* Bytes of the two buffers. */

@@ -14,9 +14,9 @@
 // own 128 rows of B, half of A's rows and all of A's scales.  A stage is 128 bytes of codes of every row: 128 values, 256 where both are e2m1;
 // e2m1 beside e4m3 is spread to a byte a value on the way into shared memory (by TMA: 16 values a 16-byte unit).
 //
-// Large products are bound by the tensor core's clock under the power cap and by the way from L2 (8192^3: 4 bits 204 to 218 us, 5.0 to 5.4 PFLOP/s; 8 bits 393
-// to 430, 2.6 to 2.8), products with few rows of A by B's bytes (16 x 16384 x 16384 in 8 bits 48.5 us, 5.7 TB/s) and small ones by latency (1 x 4096 x 4096
-// 8 by 4 bits 5.7 us).
+// Large products are bound by the tensor core's clock under the power cap and by the way from L2 (8192^3 alone: 4 bits 203 to 218 us, 5.0 to 5.4 PFLOP/s, and 244
+// to 254 among seconds of such products; 8 bits 393 to 430, 2.6 to 2.8), products with few rows of A by B's bytes (16 x 16384 x 16384 in 8 bits
+// 47.8 us, 5.8 TB/s) and small ones by latency (1 x 4096 x 4096 8 by 4 bits 5.8 us).
 #pragma once
 #include <type_traits>
 

@@ -8,7 +8,7 @@
 // A block's scale is 2^max(floor(log2 m) - e, -127), m its largest magnitude and e the exponent of the type's largest value (8, 2).  A value is
 // multiplied by the inverse, which is exact, and rounded once, to the nearest, ties to even; what would round past the type's largest
 // value is held there (m can be up to 512 in e4m3's units, whose largest value is 448, and 8 in e2m1's, whose is 6).  A block with a NaN or an
-// infinity gets the scale NaN, which turns all it meets into NaN.
+// infinity gets the scale NaN, which turns all it meets into NaN (SB200_ACT_RELU behind a product makes 0 of that, as in the other GEMMs).
 #pragma once
 #include <cuda_fp4.h>
 #include <cuda_fp8.h>
@@ -19,7 +19,6 @@
 
 namespace sb200 {
 
-constexpr int MX_BLOCK = 32;         // values that share a scale
 constexpr int MX_CHUNK = 128;        // values of a row whose scales lie side by side in a tile; K is padded to a multiple of it
 constexpr int MX_TILE_BYTES = 512;   // 128 rows x 4 scales
 

@@ -10,7 +10,7 @@
 //
 // A block a row, or a warp up to 1024 columns, the row in registers (VECS float4 a thread; thread t has columns 4 (v * threads + t)), so that x
 // and residual are read once.  Rows too long for that (32768 columns on) are read twice.  Bound by HBM: 8 bytes read, 5 written a value with
-// 8-bit codes, and by the blocks in flight: 8192 x 8192 with a residual to 8 bits takes 142 us (135 at the copy bandwidth), with 126 registers a thread
+// 8-bit codes, and by the blocks in flight: 8192 x 8192 with a residual to 8 bits takes 143 us (135 at the copy bandwidth), with 126 registers a thread
 // and one block an SM it took 337.
 #pragma once
 #include <cuda_runtime.h>

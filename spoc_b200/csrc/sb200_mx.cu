@@ -87,7 +87,7 @@ int matrix_extent(int dev, uint64_t p, int64_t rows, int64_t cols, int64_t ld, c
 // (4096 x 4096 x 2048) take 118 us instead of 107, and 2047 x 1021 to 4 bits and back 8.4 instead of 6.2.
 constexpr int kShared = 50;
 
-// Blocks for `work` units, `per_block` each, at most `waves` waves of what fits a chip.
+// Blocks for `work` units, `per_block` each, at most `cap`.
 unsigned grid_for(int64_t work, int64_t per_block, int64_t cap) {
   const int64_t blocks = (work + per_block - 1) / per_block;
   return static_cast<unsigned>(std::max<int64_t>(1, std::min(blocks, cap)));
@@ -99,7 +99,8 @@ int launch_rmsnorm(int sm_count, cudaStream_t st, const RmsNorm& p) {
   const int64_t rows = FORMAT ? (p.rows + 127) / 128 * 128 : p.rows;
   constexpr int ACCESS = VEC ? ACCESS_VECTOR : FORMAT ? ACCESS_SINGLE : ACCESS_LANES;
   // The row in the registers of a warp or a block, and as many blocks an SM as leave a thread 48 registers (64 with eight float4).  Few rows, which
-  // do not fill the chip, take wide blocks: 1 x 4096 to 8 bits 3.96 -> 3.07 us, 512 x 4096 9.7 -> 8.0, where 8192 x 4096 goes 70.8 -> 83.4.
+  // do not fill the chip, take wide blocks: 1 x 4096 to 8 bits 3.66 -> 2.93 us, 444 x 4096 9.3 -> 7.5, 444 x 1024 6.1 -> 3.0; 512 x 4096 is even,
+  // 512 x 8192 goes 15.6 -> 17.8 and 8192 x 4096 70.8 -> 83.4.
 #define SB200_NORM(THREADS, VECS, BLOCKS)                                                                                            \
   CU_TRY(launch_pdl(rmsnorm_kernel<FORMAT, THREADS, VECS, ACCESS, BLOCKS>, dim3(grid_for(rows, THREADS == 32 ? 4 : 1, 0x7fffffff)),  \
                     dim3(THREADS == 32 ? 128 : THREADS), 0, st, 1, p))

@@ -89,3 +89,20 @@ def test_rows_that_are_not_numbers_leave_what_is_past_them_zero(keep, device, co
     assert not codes[:, -(-cols // per_byte):].any()
     if cols % per_byte:
         assert not (codes[:, cols // per_byte] >> 4).any()
+
+
+def test_a_clamp_makes_zero_of_nan(keep, device):  # noqa: F811
+    """Scales of NaN show in a product, and are zeros behind SB200_ACT_RELU, as in the product of float32."""
+    a, b = np.ones((5, 64)), np.ones((7, 64))
+    a[2, 3] = np.nan
+    A, B, d = keep.mx(R.FP8, 5, 64, R.quantize(a, R.FP8)), keep.mx(R.FP4, 7, 64, R.quantize(b, R.FP4)), keep.out(35)
+    want = np.full((5, 7), 64.0)
+    for act, nan in ((0, np.nan), (1, 0.0)):
+        want[2] = nan
+        R.gemm_mx(device, A, B, d, act=act)
+        keep.backend.Device.synchronize(device)
+        assert np.array_equal(d.download().reshape(5, 7), want, equal_nan=True)
+        x, y = keep.f32(a.astype(np.float32)), keep.f32(np.ascontiguousarray(b.T).astype(np.float32))
+        assert R.L.load().sb200_gemm_f32(device.id, 0, R.L.MODE_3XTF32, 5, 7, 64, x.ptr, 64, y.ptr, 7, d.ptr, 7, 1.0, 0, 0, 0.0, 0, act) == 0
+        keep.backend.Device.synchronize(device)
+        assert np.array_equal(d.download().reshape(5, 7), want, equal_nan=True)
