@@ -443,8 +443,8 @@ SB200_API int sb200_gemm_mx(int dev, uint64_t stream, int format_a, int format_b
 /* ---- root-mean-square norm ----------------------------------------------------------------------------
  * h = x + residual (rounded to float32; residual may be 0), y = h * weight / sqrt(mean(h^2) + eps), by rows of `cols`.  Results, each
  * optional: `sum` takes h, y the float32 result, codes and scales (format SB200_MX_FP8 or SB200_MX_FP4; 0: none) the microscaled one, whose
- * codes are roundings of y in 64 bits.  sum may be x or residual, and y may be x or residual, at the same leading dimension (with another it
- * is SB200_ERR_INVALID_VALUE); sum and y are two matrices. */
+ * codes are roundings of y in 64 bits (2^128 and beyond, which float32 does not hold either, counts as infinite).  sum may be x or residual, and
+ * y may be x or residual, at the same leading dimension (with another it is SB200_ERR_INVALID_VALUE); sum and y are two matrices. */
 SB200_API int sb200_rmsnorm_f32(int dev, uint64_t stream, int64_t rows, int64_t cols, uint64_t x, int64_t ldx, uint64_t residual, int64_t ldr,
                                 uint64_t weight, double eps, uint64_t sum, int64_t lds, uint64_t y, int64_t ldy,
                                 int format, uint64_t codes, uint64_t scales);

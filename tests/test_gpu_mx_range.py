@@ -106,3 +106,20 @@ def test_a_clamp_makes_zero_of_nan(keep, device):  # noqa: F811
         assert R.L.load().sb200_gemm_f32(device.id, 0, R.L.MODE_3XTF32, 5, 7, 64, x.ptr, 64, y.ptr, 7, d.ptr, 7, 1.0, 0, 0, 0.0, 0, act) == 0
         keep.backend.Device.synchronize(device)
         assert np.array_equal(d.download().reshape(5, 7), want, equal_nan=True)
+
+
+@pytest.mark.parametrize("fmt", R.FORMATS)
+def test_norms_past_float32_are_infinite(keep, device, fmt):  # noqa: F811
+    """Weights near float32's largest: blocks with a y of 2^128 and more have the scale NaN, the others the codes of 64 bits."""
+    rng = np.random.default_rng(fmt)
+    x = rng.normal(size=(40, 320)).astype(np.float32)
+    w = np.where(np.arange(320) // 32 % 2 == 0, 3e38, 1e38).astype(np.float32)
+    _, y, (codes, scales) = run_norm(keep, device, x, None, w, 1e-5, fmt)
+    want = R.rmsnorm(x, None, w, 1e-5)[1]
+    past = np.abs(want) >= 2.0 ** 128
+    assert past.any() and np.all(np.isinf(y[past]))
+    want_codes, want_scales = R.quantize(np.where(past, np.inf, want), fmt)
+    assert 0 < (want_scales == 255).sum() < want_scales.size / 2 and np.array_equal(scales, want_scales)
+    fine = ~np.pad(past, ((0, 0), (0, 64))).reshape(40, 12, 32).any(-1)
+    per_block = 16 if fmt == R.FP4 else 32
+    assert np.array_equal(codes.reshape(40, 12, per_block)[fine], want_codes.reshape(40, 12, per_block)[fine])
